@@ -41,9 +41,10 @@ const char* svc_last_error(void);
  *      generator entry points (svc_conv1d_h*, svc_conv1d_hl*, svc_resblock_pair_h / _hl)
  *   5: SVC_MMA_BF16X6 removed (svc_conv1d_args.mma / svc_wgrad_args.mma accept fp32, bf16, fp16 only); split pipeline range guard:
  *      svc_conv1d_h_args.acc_scale, svc_pack_conv1d_hl(scale), svc_resblock_pair_hl(acc_scale1, acc_scale2), svc_hl_range_flag; svc_coupling_fused_h
+ *   7: svc_attn_scored_fwd / _bwd, svc_dropout_add_layernorm_fwd / _bwd
  *   6: svc_conv1d_args / svc_convt1d_args grew {w_d4} (lane-linear weight pack of the short-sequence kernel), svc_pack_conv1d_d4,
  *      svc_conv1d_wants_d4 */
-#define SVC_ABI_VERSION 6
+#define SVC_ABI_VERSION 7
 int svc_abi_version(void);
 /* Fills name[0..len) with the gcnArchName of the current device, returns number of CUs (or <0). */
 int svc_device_info(char* name, int len);
@@ -732,6 +733,96 @@ int svc_dft_basis_f32(float* cs, float* sn, int N, int NB, void* stream);
 int svc_cmag_f32(const float* re, const float* im, float* mag, long long n, float eps, void* stream);
 int svc_cmag_bwd_f32(const float* re, const float* im, const float* mag, const float* dmag, float* dre, float* dim, long long n,
                      void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Attention with scored options, forward and backward (modules/attentions.py:207-239 with proximal_bias :219-222,305-316 and
+ * block_length :224-229 as two of its cases), flash style: scores live in registers only.
+ *
+ * Tensors are [B, heads*dk, T] views of `dtype` (fp32, bf16 or fp16; all of one call the same), time contiguous, any element strides
+ * _bs / _cs, rows at any alignment of the type.  H query heads share G key / value heads (G divides H).  Query t of item b is
+ * position p = offset + t of the key axis (`offsets[b]` instead of `offset` when given).  With len = lengths[b] (or Tk) it sees the
+ * keys of [lo, hi):
+ *   p outside [0, len)  none
+ *   n_docs > 0          those of its document, [docs[b][n], docs[b][n+1]) with n_docs + 1 non-decreasing boundaries per item; none when
+ *                       p lies in no document
+ *   causal              s <= p, and with `prefix` also s < start + prefix (start = the document's or 0; prefix[b], or prefix[b][n]
+ *                       with documents): a bidirectional front
+ *   window >= 0         |s - p| <= window (not together with prefix); -1: none
+ * What lies at keys that no query of a tile sees (unwritten cache behind `lengths`, other documents' tails) is never used.
+ *   score = cap(scale q.k) + bias[h][clamp(s - p, -bias_w, bias_w) + bias_w],  cap(u) = softcap tanh(u / softcap) or u (softcap 0)
+ *   P = softmax over the visible keys; a query that sees none gets out = 0 and passes no gradient.
+ *   out = sum_s Z P v,  Z = keep / (1 - theta): attention dropout when seed != NULL, theta = round(65536 p_drop) / 65536 and
+ *   keep[b,h,t,s] = (field s & 3 of word((b H + h) Tq + t) ceil(Tk / 4) + (s >> 2)) >= 65536 theta), word(i) the 64-bit value whose
+ *   top 24 bits are svc_dropout_rng_f32's draw i of (seed, site), its fields 16 bits from the lowest.  Nothing is stored.
+ * bias: fp32 [bias_heads][2 bias_w + 1] contiguous, bias_heads = H or 1; its gradient dbias has the same shape (NULL: not wanted).
+ * Accumulation, softmax statistics and gradients of the bias are fp32 for every dtype; P and dS are rounded to dtype as operands.
+ *
+ * svc_attn_scored_fwd writes out and, when not NULL, lse [B,H,Tq] (log2 of the sum of exp2 of the scores in log2 units; 0 for a query
+ * without keys) and out32 [B,H*dk,Tq], contiguous: the output in fp32, for which P goes into the product as two operands of a 16-bit type
+ * (its square's rounding instead of its own).  svc_attn_scored_bwd reads q, k, v, out32 (or out, when out32 is NULL), lse, dout and
+ * writes dq, dk, dv (contiguous [B, heads*dk, T]) and dbias.  The rows' sums of dO out enter dbias unrounded, so 16-bit types' dbias, an fp32
+ * result, wants out32.  No atomics on memory: results do not vary from run to run.  ws: svc_attn_scored_ws_bytes(a, backward) bytes, 16-byte aligned, contents undefined before and after.
+ * Built for 1 <= dk <= 128, 0 <= Tq <= Tk < 2^30.
+ * ---------------------------------------------------------------------------------------------- */
+enum { SVC_F32 = 0, SVC_BF16 = 1, SVC_F16 = 2 };
+typedef struct svc_attn_scored_t {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* out32;
+  float* lse;
+  const float* bias;
+  const int* lengths;  /* [B] or NULL */
+  const int* offsets;  /* [B] or NULL */
+  const int* docs;     /* [B][n_docs + 1] or NULL */
+  const int* prefix;   /* [B] ([B][n_docs] with documents) or NULL */
+  const long long* seed; /* int64[1] or NULL: no dropout */
+  const void* dout;
+  void* dq;
+  void* dk_;
+  void* dv;
+  float* dbias;
+  void* ws;
+  long long ws_bytes;
+  long long q_bs, q_cs, k_bs, k_cs, v_bs, v_cs, o_bs, o_cs, do_bs, do_cs;
+  int dtype, B, H, G, dk, Tq, Tk;
+  int causal, window, n_docs, offset, bias_w, bias_heads, site;
+  float scale, softcap, p_drop;
+} svc_attn_scored_t;
+long long svc_attn_scored_ws_bytes(const svc_attn_scored_t* a, int backward);
+int svc_attn_scored_fwd(const svc_attn_scored_t* a, void* stream);
+int svc_attn_scored_bwd(const svc_attn_scored_t* a, void* stream);
+
+/* The residual junction of a transformer layer: y = LayerNorm_C(r + dropout(x)) * gamma + beta, times mask (modules/attentions.py:51-55,
+ * 100-104 with modules/modules.py:23-35), forward and backward.  x, r, y, dy, dx, dr: [B, C, T] of `dtype`, contiguous; gamma, beta,
+ * dgamma, dbeta: fp32 [C]; mean, rstd: fp32 [B, T] (forward: written when not NULL); mask: fp32 [B, T] or NULL — where it is 0, y and every
+ * gradient are 0 whatever x and r hold there.  r may be NULL.  seed != NULL: dropout of x with svc_dropout_rng_f32's draws of (seed, site) and
+ * rate p, recomputed in the backward.  Statistics, sums and gradients in fp32 (the parameters' in fixed order, no atomics).
+ * Backward: dx may be NULL (no dropout: it equals dr).  ws: svc_dropout_add_layernorm_ws_bytes(C, B, T) bytes, 16-byte aligned. */
+typedef struct svc_dropout_add_layernorm_t {
+  const void* x;
+  const void* r;
+  const float* gamma;
+  const float* beta;
+  const float* mask;
+  void* y;
+  float* mean;
+  float* rstd;
+  const long long* seed;
+  const void* dy;
+  void* dx;
+  void* dr;
+  float* dgamma;
+  float* dbeta;
+  void* ws;
+  long long ws_bytes;
+  int dtype, B, C, T, site;
+  float p, eps;
+} svc_dropout_add_layernorm_t;
+long long svc_dropout_add_layernorm_ws_bytes(int B, int C, int T);
+int svc_dropout_add_layernorm_fwd(const svc_dropout_add_layernorm_t* a, void* stream);
+int svc_dropout_add_layernorm_bwd(const svc_dropout_add_layernorm_t* a, void* stream);
 
 /* Tuning / debugging knob of svc_conv1d_f32 (tile-config override and ablation switches); 0 restores defaults. */
 int svc_debug_set_conv_cfg(int cfg);

@@ -1,0 +1,202 @@
+// attn_scored_fwd.hip — svc_attn_scored_fwd: attention with capped scores, distance bias, document / prefix / window masks and
+// counter-based dropout; one pass over the keys with a running maximum and sum per query.
+#include "attn_scored.h"
+
+namespace attn {
+
+// A workgroup owns 128 queries of one head (32 a wave) and walks the key tiles that any of them sees.
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void fwd_kernel(svc_attn_scored_t a, int n_tiles) {
+  constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
+  __shared__ __align__(16) char ks_[DP * PITCH], vs_[DP * PITCH];
+  __shared__ float win[NCOL + N];
+  __shared__ int range[2][4];
+  E* ks = (E*)ks_;
+  E* vs = (E*)vs_;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, n = lane & 31;
+  const int bh = blockIdx.x / n_tiles, t0 = (blockIdx.x % n_tiles) * NCOL;
+  const int b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.G);
+  const E* kp = (const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs;
+  const E* vp = (const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs;
+  const E* qp = (const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs;
+
+  const int tl = wave * 32 + n, t = t0 + tl;
+  const int len = item_length(a, b), off = item_offset(a, b);
+  int2 iv = make_int2(0, 0);
+  if (t < a.Tq && (!a.offsets || (off >= -a.Tq && off < a.Tk))) iv = visible(a, b, len, off + t);
+  // the wave's and the workgroup's key range, and the range that every query of the wave sees whole
+  const bool some = iv.y > iv.x;
+  const int wlo = wave_min(some ? iv.x : a.Tk), whi = wave_max(iv.y);
+  const int flo = wave_max(t < a.Tq ? (some ? iv.x : a.Tk) : 0), fhi = wave_min(t < a.Tq ? iv.y : a.Tk);
+  if (lane == 0) {
+    range[0][wave] = wlo;
+    range[1][wave] = whi;
+  }
+  __syncthreads();
+  const int blo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3]));
+  const int bhi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
+
+  typename Frag<E>::template Head<DP> q;
+  load_columns<E, DP>(q, qp, a.q_cs, a.dk, t, a.Tq, h);
+  const ScoreScale sc = score_scale(a);
+  const float* table = a.bias ? a.bias + (a.bias_heads > 1 ? (long long)head * (2 * a.bias_w + 1) : 0) : nullptr;
+  unsigned long long draws = 0;
+  unsigned thr = 0;
+  if (a.seed) {
+    const unsigned long long row = ((unsigned long long)b * a.H + head) * a.Tq + t;
+    draws = draw_start(a) + row * (unsigned long long)((a.Tk + 3) >> 2) * 0xD1B54A32D192ED03ull;
+    thr = (unsigned)rintf(a.p_drop * 65536.f);
+  }
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  for (int s0 = blo / N * N; s0 < bhi; s0 += N) {
+    __syncthreads();
+    stage<E, DP>(ks, kp, a.k_cs, a.dk, s0, blo, bhi, tid);
+    stage<E, DP>(vs, vp, a.v_cs, a.dk, s0, blo, bhi, tid);
+    if (table) stage_bias(win, table, a.bias_w, s0 - (off + t0) - (NCOL - 1), NCOL + N, tid);
+    __syncthreads();
+    if (s0 >= whi || s0 + N <= wlo) continue;
+    float s[RT][16];
+    float mt = -INFINITY;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      f32x16 u;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) u[r] = 0.f;
+      u = mul_columns<E, DP>(ks, rt, q, u, lane);
+      if (sc.cap_in > 0.f) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[rt][r] = tanhf(u[r] * sc.cap_in) * sc.cap_out;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[rt][r] = u[r] * sc.mul;
+      }
+      if (table) {
+        const float* w = win + 32 * rt + (NCOL - 1) - tl;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[rt][r] += w[pos_of(r, h)];
+      }
+      if (s0 < flo || s0 + N > fhi) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int p = s0 + 32 * rt + pos_of(r, h);
+          s[rt][r] = p >= iv.x && p < iv.y ? s[rt][r] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[rt][r]);
+    }
+    mt = fmaxf(mt, __shfl_xor(mt, 32));
+    const float m1 = fmaxf(m, mt), ms = m1 == -INFINITY ? 0.f : m1 - PUP<E>;
+    const float alpha = __builtin_amdgcn_exp2f(m - (ms + PUP<E>));
+    m = m1;
+    l *= alpha;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[rt][r] = __builtin_amdgcn_exp2f(s[rt][r] - ms);
+        l += s[rt][r];
+      }
+      if (a.seed) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const unsigned long long z = draw_word(draws, (unsigned long long)((s0 + 32 * rt + pos_of(4 * w, h)) >> 2));
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (((unsigned)(z >> (16 * j)) & 0xffffu) < thr) s[rt][4 * w + j] = 0.f;
+        }
+      }
+      if (sizeof(E) == 2 && a.out32) mul_rows<E, DP, true>(acc, vs, rt, s[rt], lane);
+      else mul_rows<E, DP>(acc, vs, rt, s[rt], lane);
+    }
+  }
+
+  l += __shfl_xor(l, 32);
+  if (t >= a.Tq) return;
+  float inv = l > 0.f ? 1.f / l : 0.f;
+  if (l != l) inv = l;                                  // nan scores give nan, as they would in any softmax
+  if (a.seed) inv *= 65536.f / (65536.f - (float)thr);
+  if (a.lse && h == 0) a.lse[(long long)bh * a.Tq + t] = some ? m - PUP<E> + __builtin_amdgcn_logf(l) : 0.f;
+  E* op = (E*)a.out + b * a.o_bs + (long long)head * a.dk * a.o_cs + t;
+  float* fp = a.out32 ? a.out32 + (long long)bh * a.dk * a.Tq + t : nullptr;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int d = 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
+      if (d < a.dk) {
+        const float v = acc[i][r] * inv;
+        op[d * a.o_cs] = (E)v;
+        if (fp) fp[(long long)d * a.Tq] = v;
+      }
+    }
+}
+
+int check_args(const svc_attn_scored_t* a, bool backward) {
+  SVC_REQUIRE(a, "attn_scored: no arguments");
+  SVC_REQUIRE(a->dtype >= 0 && a->dtype <= 2, "attn_scored: dtype %d", a->dtype);
+  SVC_REQUIRE(a->B >= 0 && a->Tq >= 0 && a->Tq <= a->Tk && a->Tk < (1 << 30), "attn_scored: B=%d Tq=%d Tk=%d (0 <= Tq <= Tk < 2^30)",
+              a->B, a->Tq, a->Tk);
+  SVC_REQUIRE(a->G >= 1 && a->H >= a->G && a->H % a->G == 0, "attn_scored: %d query heads, %d key heads", a->H, a->G);
+  SVC_REQUIRE(a->dk >= 1 && a->dk <= 128, "attn_scored: head size %d (1..128)", a->dk);
+  SVC_REQUIRE(a->offsets || (a->offset >= 0 && a->offset <= a->Tk - a->Tq), "attn_scored: offset %d with Tq=%d Tk=%d", a->offset, a->Tq, a->Tk);
+  SVC_REQUIRE(a->window >= -1 && a->n_docs >= 0 && (a->n_docs == 0 || a->docs), "attn_scored: window %d, %d documents", a->window, a->n_docs);
+  SVC_REQUIRE(!a->prefix || (a->causal && a->window < 0), "attn_scored: a prefix goes with a causal mask and no window");
+  SVC_REQUIRE(!a->bias || (a->bias_w >= 0 && a->bias_w < (1 << 29) && (a->bias_heads == 1 || a->bias_heads == a->H)),
+              "attn_scored: bias of %d heads, width %d", a->bias_heads, a->bias_w);
+  SVC_REQUIRE(a->scale == a->scale && a->softcap >= 0.f && a->softcap < INFINITY, "attn_scored: scale %g, softcap %g", a->scale, a->softcap);
+  SVC_REQUIRE(!a->seed || (a->p_drop >= 0.f && a->p_drop <= 0.99f), "attn_scored: dropout rate %g (0..0.99)", a->p_drop);
+  if (a->B == 0 || a->Tq == 0) return SVC_OK;
+  SVC_REQUIRE(a->q && a->k && a->v, "attn_scored: q, k, v");
+  if (!backward) SVC_REQUIRE(a->out, "attn_scored: out");
+  if (backward) {
+    SVC_REQUIRE(a->dout && a->lse && a->dq && a->dk_ && a->dv && (a->out || a->out32), "attn_scored_bwd: dout, lse, out or out32, dq, dk, dv");
+    SVC_REQUIRE(!a->dbias || (a->bias && (a->dtype == SVC_F32 || a->out32)), "attn_scored_bwd: dbias needs bias, and out32 for 16-bit types");
+  }
+  const long long need = svc_attn_scored_ws_bytes(a, backward);
+  SVC_REQUIRE(need == 0 || (a->ws && a->ws_bytes >= need && ((size_t)a->ws & 15) == 0), "attn_scored: workspace of %lld bytes needed, %lld given",
+              need, a->ws ? a->ws_bytes : 0LL);
+  const long long groups = (long long)a->B * a->H * svc::cdiv(a->Tk, 32);
+  SVC_REQUIRE(groups < (1LL << 31), "attn_scored: %lld tiles", groups);
+  return SVC_OK;
+}
+
+template <typename E, int DP>
+static void launch_fwd(const svc_attn_scored_t& a, hipStream_t s) {
+  const int n_tiles = (a.Tq + NCOL - 1) / NCOL;
+  hipLaunchKernelGGL((fwd_kernel<E, DP>), dim3((unsigned)(a.B * a.H * n_tiles)), dim3(256), 0, s, a, n_tiles);
+}
+template <typename E>
+static void pick_fwd(const svc_attn_scored_t& a, hipStream_t s) {
+  if (a.dk <= 32) launch_fwd<E, 32>(a, s);
+  else if (a.dk <= 64) launch_fwd<E, 64>(a, s);
+  else if (a.dk <= 96) launch_fwd<E, 96>(a, s);
+  else launch_fwd<E, 128>(a, s);
+}
+
+}  // namespace attn
+
+extern "C" {
+
+int svc_attn_scored_fwd(const svc_attn_scored_t* a, void* stream) {
+  const int rc = attn::check_args(a, false);
+  if (rc != SVC_OK || a->B == 0 || a->Tq == 0) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  svc::ProfScope prof(s, "attn_scored_fwd", 4.0 * a->B * a->H * (double)a->Tq * a->Tk * a->dk, 0);
+  if (a->dtype == SVC_F32) attn::pick_fwd<float>(*a, s);
+  else if (a->dtype == SVC_BF16) attn::pick_fwd<attn::bf16_t>(*a, s);
+  else attn::pick_fwd<attn::f16_t>(*a, s);
+  return svc::check_launch("svc_attn_scored_fwd");
+}
+
+}  // extern "C"

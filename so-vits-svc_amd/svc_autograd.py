@@ -15,6 +15,7 @@ import math
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 import svc_hip as S
 
@@ -1009,6 +1010,63 @@ class _AttentionQKV(Function):
 def attention_qkv(qkv, n_heads, emb_rel_k=None, emb_rel_v=None, window=0, mask=None, mask_mode=0, drop_u=None, p_drop=0.0):
     """attention() on a fused [B, 3C, T] projection whose rows are ordered (head, {q, k, v}, d) — see _AttentionQKV."""
     return _AttentionQKV.apply(qkv, emb_rel_k, emb_rel_v, mask, n_heads, window or 0, mask_mode, drop_u, float(p_drop))
+
+
+class _AttentionScored(Function):
+    """svc_hip.attention_scored with its gradients; nothing of [Tq, Tk] is kept, attention dropout is redrawn in the backward."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bias, n_heads, opts, sides, draw):
+        out, lse, out32 = S.attention_scored_fwd(q, k, v, n_heads, bias=bias, draw=draw, want_dbias=ctx.needs_input_grad[3], **opts, **sides)
+        ctx.save_for_backward(q, k, v, bias, lse, out if out32 is None else out32, *sides.values())
+        ctx.cfg = (n_heads, opts, list(sides), draw)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, bias, lse, out, *sides = ctx.saved_tensors
+        n_heads, opts, names, draw = ctx.cfg
+        dq, dk, dv, dbias = S.attention_scored_bwd(dout, q, k, v, out, lse, n_heads, bias=bias, draw=draw, want_dbias=ctx.needs_input_grad[3],
+                                                   **opts, **dict(zip(names, sides)))
+        return dq, dk, dv, dbias, None, None, None, None
+
+
+def attention_scored(q, k, v, n_heads, *, bias=None, softcap=0.0, scale=None, causal=False, window=None, prefix=None, docs=None, lengths=None,
+                     offset=None, draw=None, p_drop=0.0):
+    """svc_hip.attention_scored for training: gradients of q, k, v and the distance bias; `draw` (a svc_hip.HashDraw, whose seed stays put until
+    the backward has run) and `p_drop`: dropout of the attention probabilities."""
+    opts = dict(softcap=softcap, scale=scale, causal=causal, window=window, p_drop=float(p_drop))
+    sides = {n: t for n, t in (("prefix", prefix), ("docs", docs), ("lengths", lengths)) if t is not None}
+    if isinstance(offset, torch.Tensor):
+        sides["offset"] = offset
+    else:
+        opts["offset"] = offset
+    return _AttentionScored.apply(q, k, v, bias, n_heads, opts, sides, draw)
+
+
+class _DropoutAddLayerNorm(Function):
+    """svc_hip.dropout_add_layernorm with its gradients; r + dropout(x) is recomputed in the backward."""
+
+    @staticmethod
+    def forward(ctx, x, r, gamma, beta, mask, draw, p, eps):
+        y, mean, rstd = S.dropout_add_layernorm(x, r, gamma, beta, draw=draw, p=p, mask=mask, eps=eps, stats=True)
+        ctx.save_for_backward(x, r, gamma, beta, mean, rstd, mask)
+        ctx.cfg = (draw, p, eps)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, r, gamma, beta, mean, rstd, mask = ctx.saved_tensors
+        draw, p, eps = ctx.cfg
+        dx, dr, dgamma, dbeta = S.dropout_add_layernorm_bwd(dy, x, r, gamma, beta, mean, rstd, draw=draw, p=p, mask=mask, eps=eps)
+        return dx, dr, dgamma, dbeta, None, None, None, None
+
+
+def dropout_add_layernorm(x, r, gamma, beta, *, draw=None, p=0.0, mask=None, eps=1e-5):
+    """svc_hip.dropout_add_layernorm for training: gradients of x, r (may be None), gamma and beta."""
+    return _DropoutAddLayerNorm.apply(x, r, gamma, beta, mask, draw, float(p), float(eps))
 
 
 class _Dropout(Function):

@@ -116,6 +116,19 @@ class AttentionArgs(C.Structure):
     ]
 
 
+class AttnScored(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "out32", "lse", "bias", "lengths", "offsets", "docs", "prefix", "seed", "dout",
+                                          "dq", "dk_", "dv", "dbias", "ws")] + \
+        [(n, C.c_longlong) for n in ("ws_bytes", "q_bs", "q_cs", "k_bs", "k_cs", "v_bs", "v_cs", "o_bs", "o_cs", "do_bs", "do_cs")] + \
+        [(n, C.c_int) for n in ("dtype", "B", "H", "G", "dk", "Tq", "Tk", "causal", "window", "n_docs", "offset", "bias_w", "bias_heads", "site")] + \
+        [(n, C.c_float) for n in ("scale", "softcap", "p_drop")]
+
+
+class DropoutAddLayernorm(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "r", "gamma", "beta", "mask", "y", "mean", "rstd", "seed", "dy", "dx", "dr", "dgamma", "dbeta", "ws")] + \
+        [("ws_bytes", C.c_longlong)] + [(n, C.c_int) for n in ("dtype", "B", "C", "T", "site")] + [("p", C.c_float), ("eps", C.c_float)]
+
+
 _lib = None
 
 
@@ -196,6 +209,14 @@ def lib():
             [C.c_int] * 3 + [C.c_void_p]
         L.svc_posconv_pack_f32.argtypes = [_f32p, _f32p, _f32p, C.c_int, C.c_int, C.c_int, C.c_void_p]
         L.svc_posconv_f32.argtypes = [_f32p] * 4 + [C.c_int] * 6 + [C.c_void_p]
+        L.svc_attn_scored_ws_bytes.argtypes = [C.POINTER(AttnScored), C.c_int]
+        L.svc_attn_scored_ws_bytes.restype = C.c_longlong
+        for fn in (L.svc_attn_scored_fwd, L.svc_attn_scored_bwd):
+            fn.argtypes = [C.POINTER(AttnScored), C.c_void_p]
+        L.svc_dropout_add_layernorm_ws_bytes.argtypes = [C.c_int] * 3
+        L.svc_dropout_add_layernorm_ws_bytes.restype = C.c_longlong
+        for fn in (L.svc_dropout_add_layernorm_fwd, L.svc_dropout_add_layernorm_bwd):
+            fn.argtypes = [C.POINTER(DropoutAddLayernorm), C.c_void_p]
         L.svc_debug_set_conv_strip.argtypes = [C.c_int]
         if os.environ.get("SVC_CONV_STRIP"):     # A/B switch of the strip kernel (csrc/conv1d_strip.hip), read once at load
             L.svc_debug_set_conv_strip(int(os.environ["SVC_CONV_STRIP"]))
@@ -203,7 +224,7 @@ def lib():
     return _lib
 
 
-ABI_VERSION = 6      # include/svc_hip.h SVC_ABI_VERSION (tests/test_abi_cpu.py keeps the two and the struct layouts in step)
+ABI_VERSION = 7      # include/svc_hip.h SVC_ABI_VERSION (tests/test_abi_cpu.py keeps the two and the struct layouts in step)
 
 EXPORTS = [
     "svc_last_error", "svc_abi_version", "svc_device_info", "svc_debug_empty_kernel", "svc_prof_enable", "svc_prof_reset", "svc_prof_report",
@@ -213,6 +234,8 @@ EXPORTS = [
     "svc_conv1d_direct_f32", "svc_resblock_pair_f32", "svc_resblock16_f32", "svc_nsf_source_scratch_bytes", "svc_nsf_source_f32", "svc_f0_to_coarse",
     "svc_prenet_embed_f32", "svc_add_layernorm_f32", "svc_reparam_f32", "svc_attention_f32", "svc_attention_ws_bytes", "svc_pack_conv1d_h", "svc_conv1d_h", "svc_resblock_pair_h", "svc_snake_alias_h", "svc_debug_set_conv_h", "svc_cvt_to_h", "svc_cvt_from_h", "svc_conv_post_h", "svc_hl_range_flag", "svc_coupling_fused_h", "svc_debug_set_coupling_fused", "svc_pack_conv1d_hl", "svc_conv1d_hl", "svc_debug_set_conv_hl", "svc_resblock_pair_hl", "svc_snake_alias_hl", "svc_cvt_to_hl", "svc_cvt_from_hl", "svc_conv_post_hl", "svc_debug_set_attention_waves", "svc_posconv_pack_f32", "svc_posconv_f32", "svc_copy_bct_f32", "svc_f0_norm_lf0_f32", "svc_lf0_to_f0_f32",
     "svc_resample_sinc_f32", "svc_snake_alias_f32", "svc_snake_alias_bwd_f32", "svc_channel_norm_gelu_f32", "svc_channel_norm_gelu_len_f32", "svc_nsf_source_exact_f32", "svc_sinusoidal_emb_f32",
+    "svc_attn_scored_ws_bytes", "svc_attn_scored_fwd", "svc_attn_scored_bwd",
+    "svc_dropout_add_layernorm_ws_bytes", "svc_dropout_add_layernorm_fwd", "svc_dropout_add_layernorm_bwd",
 ]
 
 
@@ -1984,3 +2007,250 @@ def cmag_bwd(re, im, mag, dmag):
     check(t2lib().svc_cmag_bwd_f32(ptr(re), ptr(im), ptr(mag), ptr(dmag.contiguous()), ptr(dre), ptr(dim), re.numel(),
                                    stream_ptr()), "cmag_bwd")
     return dre, dim
+
+
+# --------------------------------------------------------------------------------------------------------------
+# transformer-layer operators on [B, C, T] tensors of any of the three types: attention with scored options, and the
+# dropout + residual + LayerNorm junction (include/svc_hip.h: svc_attn_scored_fwd / _bwd, svc_dropout_add_layernorm_fwd / _bwd)
+# --------------------------------------------------------------------------------------------------------------
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _launch_on(dev, fn, args, what):
+    """fn(args, stream) on `dev`'s current stream, whatever the current device is."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(C.byref(args), torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(C.byref(args), torch.cuda.current_stream().cuda_stream)
+    if rc:
+        check(rc, what)
+
+
+def _typed(what, *tensors):
+    """The tensors are on one GPU and of one of the three types; -> (device, type code)."""
+    t0 = tensors[0]
+    if t0.dtype not in _DTYPE:
+        raise SvcError(f"{what}: fp32, bf16 or fp16 tensors; got {t0.dtype}")
+    for t in tensors:
+        if not t.is_cuda:
+            raise SvcError(f"{what}: tensors on the GPU (cuda:N on ROCm); there is no CPU fallback")
+        if t.dtype != t0.dtype or t.device != t0.device:
+            raise SvcError(f"{what}: one type and device for all tensors; got {t0.dtype} on {t0.device} and {t.dtype} on {t.device}")
+    return t0.device, _DTYPE[t0.dtype]
+
+
+def _side(what, name, t, shape, dtype, dev):
+    """A side input (mask, lengths, table, parameter) of exact shape and type, contiguous on `dev`; -> its address."""
+    if t.dtype != dtype or t.device != dev or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise SvcError(f"{what}: {name} must be a contiguous {dtype} tensor {tuple(shape)} on {dev}; got {t.dtype} {tuple(t.shape)} on {t.device}"
+                       f"{'' if t.is_contiguous() else ', not contiguous'}")
+    return t.data_ptr()
+
+
+def _drop_args(what, a, draw, p, dev):
+    if not 0.0 <= p < 1.0:
+        raise SvcError(f"{what}: dropout rate {p}")
+    if p > 0.0:
+        if not isinstance(draw, HashDraw):
+            raise SvcError(f"{what}: dropout needs a svc_hip.HashDraw (the draws are recomputed, never stored)")
+        if draw.seed.device != dev:
+            raise SvcError(f"{what}: the draw's seed is on {draw.seed.device}, the tensors on {dev}")
+        a.seed, a.site = draw.seed.data_ptr(), draw.site
+        return True
+    return False
+
+
+def _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, draw, p_drop):
+    what = "attention_scored"
+    dev, code = _typed(what, q, k, v)
+    a = AttnScored()
+    (a.q_bs, a.q_cs), (a.k_bs, a.k_cs), (a.v_bs, a.v_cs) = _bct_strides(q), _bct_strides(k), _bct_strides(v)
+    B, Cq, Tq = q.shape
+    Tk = k.shape[2]
+    if n_heads < 1 or Cq % n_heads or Cq == 0:
+        raise SvcError(f"{what}: {Cq} channels do not split into {n_heads} heads")
+    dk = Cq // n_heads
+    if k.shape != v.shape or k.shape[0] != B or k.shape[1] % dk or k.shape[1] == 0 or n_heads % (k.shape[1] // dk):
+        raise SvcError(f"{what}: q {tuple(q.shape)} in {n_heads} heads of {dk}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if dk > 128:
+        raise SvcError(f"{what}: head size {dk}; built for 1..128")
+    if Tq > Tk:
+        raise SvcError(f"{what}: {Tq} queries, {Tk} keys: the queries are positions of the key axis")
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.dtype, a.B, a.H, a.G, a.dk, a.Tq, a.Tk = code, B, n_heads, k.shape[1] // dk, dk, Tq, Tk
+    a.scale = dk ** -0.5 if scale is None else scale
+    a.softcap, a.causal = softcap or 0.0, 1 if causal else 0
+    a.window = -1 if window is None else window
+    if window is not None and window < 0:
+        raise SvcError(f"{what}: window {window}")
+    if offset is None:
+        a.offset = Tk - Tq
+    elif isinstance(offset, torch.Tensor):
+        a.offsets = _side(what, "offset", offset, (B,), torch.int32, dev)
+    else:
+        if not 0 <= offset <= Tk - Tq:
+            raise SvcError(f"{what}: offset {offset} with {Tq} queries and {Tk} keys")
+        a.offset = offset
+    if lengths is not None:
+        a.lengths = _side(what, "lengths", lengths, (B,), torch.int32, dev)
+    if docs is not None:
+        if docs.dim() != 2 or docs.shape[1] < 2:
+            raise SvcError(f"{what}: docs are boundaries [B, N + 1]; got {tuple(docs.shape)}")
+        a.n_docs = docs.shape[1] - 1
+        a.docs = _side(what, "docs", docs, (B, a.n_docs + 1), torch.int32, dev)
+    if prefix is not None:
+        if not causal or window is not None:
+            raise SvcError(f"{what}: a prefix goes with causal=True and no window")
+        a.prefix = _side(what, "prefix", prefix, (B, a.n_docs) if a.n_docs else (B,), torch.int32, dev)
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[0] not in (1, n_heads) or bias.shape[1] % 2 == 0:
+            raise SvcError(f"{what}: bias [{n_heads} or 1, 2 W + 1]; got {tuple(bias.shape)}")
+        a.bias_heads, a.bias_w = bias.shape[0], bias.shape[1] // 2
+        a.bias = _side(what, "bias", bias, bias.shape, torch.float32, dev)
+    if p_drop and _drop_args(what, a, draw, p_drop, dev):
+        a.p_drop = p_drop
+    return a, dev
+
+
+def attention_scored(q, k, v, n_heads, *, bias=None, softcap=0.0, scale=None, causal=False, window=None, prefix=None, docs=None, lengths=None,
+                     offset=None, out=None):
+    """Attention with scored options (include/svc_hip.h: svc_attn_scored_fwd), forward: q [B, H*dk, Tq], k / v [B, G*dk, Tk] (G key heads shared by
+    H / G query heads each), fp32, bf16 or fp16 views with contiguous time -> [B, H*dk, Tq].
+
+    Queries are positions `offset` .. `offset + Tq - 1` of the key axis (int, or int32 [B]; default: the last Tq).  `lengths` int32 [B]: the
+    valid positions of each item.  `docs` int32 [B, N + 1]: boundaries of packed documents.  `causal`, with `prefix` (int32 [B], or [B, N] with
+    documents) a bidirectional front; `window`: |s - p| <= window.  `softcap`: scores capped to softcap * tanh(score / softcap).  `bias` fp32
+    [H or 1, 2 W + 1]: added by distance, clamped to +-W.  A query that sees no key gives 0."""
+    a, dev = _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, None, 0.0)
+    if out is None:
+        out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    else:
+        _typed("attention_scored", q, out)
+        if out.shape != q.shape:
+            raise SvcError(f"attention_scored: out {tuple(out.shape)} for q {tuple(q.shape)}")
+    a.out = out.data_ptr()
+    a.o_bs, a.o_cs = _bct_strides(out)
+    ws = _scored_ws(a, 0, dev)
+    _launch_on(dev, lib().svc_attn_scored_fwd, a, "attention_scored")
+    return out
+
+
+def _scored_ws(a, backward, dev):
+    n = lib().svc_attn_scored_ws_bytes(C.byref(a), backward)
+    if n:
+        ws = torch.empty((n,), device=dev, dtype=torch.uint8)
+        a.ws, a.ws_bytes = ws.data_ptr(), n
+        return ws
+
+
+def attention_scored_fwd(q, k, v, n_heads, *, bias=None, softcap=0.0, scale=None, causal=False, window=None, prefix=None, docs=None, lengths=None,
+                         offset=None, draw=None, p_drop=0.0, want_dbias=False):
+    """The forward of a training pass: attention_scored with attention dropout (`draw`: a HashDraw) -> (out, lse, out32), for
+    attention_scored_bwd.  out32, the unrounded output, is made for 16-bit tensors when the bias's gradient will be wanted, else None."""
+    a, dev = _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, draw, p_drop)
+    out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    lse = torch.empty((a.B, n_heads, a.Tq), device=dev, dtype=torch.float32)
+    out32 = None
+    if want_dbias and q.dtype != torch.float32:
+        out32 = torch.empty(q.shape, device=dev, dtype=torch.float32)
+        a.out32 = out32.data_ptr()
+    a.out, a.lse = out.data_ptr(), lse.data_ptr()
+    a.o_bs, a.o_cs = _bct_strides(out)
+    ws = _scored_ws(a, 0, dev)
+    _launch_on(dev, lib().svc_attn_scored_fwd, a, "attention_scored_fwd")
+    return out, lse, out32
+
+
+def attention_scored_bwd(dout, q, k, v, out, lse, n_heads, *, bias=None, softcap=0.0, scale=None, causal=False, window=None, prefix=None, docs=None,
+                         lengths=None, offset=None, draw=None, p_drop=0.0, want_dbias=False):
+    """Gradients of attention_scored_fwd -> (dq, dk, dv, dbias or None).  `out`: its output, out32 where it made one."""
+    a, dev = _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, draw, p_drop)
+    _typed("attention_scored_bwd", q, dout)
+    if dout.shape != q.shape:
+        raise SvcError(f"attention_scored_bwd: dout {tuple(dout.shape)} for q {tuple(q.shape)}")
+    if dout.shape[2] > 1 and dout.stride(2) != 1:
+        dout = dout.contiguous()
+    o = _side("attention_scored_bwd", "out", out, q.shape, torch.float32 if want_dbias else out.dtype, dev)
+    a.lse = _side("attention_scored_bwd", "lse", lse, (a.B, n_heads, a.Tq), torch.float32, dev)
+    if out.dtype == q.dtype:
+        a.out = o
+        a.o_bs, a.o_cs = _bct_strides(out)
+    elif out.dtype == torch.float32:
+        a.out32 = o
+    else:
+        raise SvcError(f"attention_scored_bwd: out is {out.dtype}, the tensors {q.dtype}")
+    a.dout = dout.data_ptr()
+    a.do_bs, a.do_cs = _bct_strides(dout)
+    if a.B == 0 or a.Tq == 0:
+        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(bias) if want_dbias else None
+    dq, dk, dv = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
+    a.dq, a.dk_, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    dbias = None
+    if want_dbias:
+        dbias = torch.empty(bias.shape, device=dev, dtype=torch.float32)
+        a.dbias = dbias.data_ptr()
+    ws = _scored_ws(a, 1, dev)
+    _launch_on(dev, lib().svc_attn_scored_bwd, a, "attention_scored_bwd")
+    return dq, dk, dv, dbias
+
+
+def _junction_args(x, r, gamma, beta, mask, draw, p, eps):
+    what = "dropout_add_layernorm"
+    dev, code = _typed(what, x, r) if r is not None else _typed(what, x)
+    if x.dim() != 3 or x.shape[1] == 0 or (r is not None and r.shape != x.shape):
+        raise SvcError(f"{what}: x {tuple(x.shape)}, r {None if r is None else tuple(r.shape)}; two [B, C, T] tensors of one shape")
+    a = DropoutAddLayernorm()
+    B, Cc, T = x.shape
+    if B > 65535:
+        raise SvcError(f"{what}: batch of {B}; built for up to 65535")
+    a.gamma, a.beta = _side(what, "gamma", gamma, (Cc,), torch.float32, dev), _side(what, "beta", beta, (Cc,), torch.float32, dev)
+    if mask is not None:
+        if mask.dim() == 3 and mask.shape[1] == 1:
+            mask = mask[:, 0]
+        a.mask = _side(what, "mask", mask, (B, T), torch.float32, dev)
+    if not eps > 0.0:
+        raise SvcError(f"{what}: eps {eps}")
+    a.dtype, a.B, a.C, a.T, a.eps = code, B, Cc, T, eps
+    if p and _drop_args(what, a, draw, p, dev):
+        a.p = p
+    return a, dev
+
+
+def dropout_add_layernorm(x, r, gamma, beta, *, draw=None, p=0.0, mask=None, eps=1e-5, stats=False):
+    """y = LayerNorm_C(r + dropout(x)) * gamma + beta, times mask: the residual junction of a transformer layer on [B, C, T] (fp32, bf16 or fp16; gamma,
+    beta fp32 [C]; mask fp32 [B, T] or [B, 1, T]; r may be None).  `draw` / `p`: dropout with svc_dropout_rng's draws.  `stats`: also return mean and
+    rstd [B, T] for dropout_add_layernorm_bwd."""
+    a, dev = _junction_args(x, r, gamma, beta, mask, draw, p, eps)
+    x, r = x.contiguous(), None if r is None else r.contiguous()
+    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    a.x, a.r, a.y = x.data_ptr(), None if r is None else r.data_ptr(), y.data_ptr()
+    if stats:
+        st = torch.empty((2, a.B, a.T), device=dev, dtype=torch.float32)
+        a.mean, a.rstd = st[0].data_ptr(), st[1].data_ptr()
+    _launch_on(dev, lib().svc_dropout_add_layernorm_fwd, a, "dropout_add_layernorm")
+    return (y, st[0], st[1]) if stats else y
+
+
+def dropout_add_layernorm_bwd(dy, x, r, gamma, beta, mean, rstd, *, draw=None, p=0.0, mask=None, eps=1e-5):
+    """Gradients of dropout_add_layernorm -> (dx, dr, dgamma, dbeta); without dropout dx and dr are one tensor, without r dr is None."""
+    what = "dropout_add_layernorm_bwd"
+    a, dev = _junction_args(x, r, gamma, beta, mask, draw, p, eps)
+    _typed(what, x, dy)
+    if dy.shape != x.shape:
+        raise SvcError(f"{what}: dy {tuple(dy.shape)} for x {tuple(x.shape)}")
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
+    if x.numel() == 0:
+        return torch.zeros_like(x), None if r is None else torch.zeros_like(x), dgamma.zero_(), dbeta.zero_()
+    x, dy, r = x.contiguous(), dy.contiguous(), None if r is None else r.contiguous()
+    a.x, a.r, a.dy = x.data_ptr(), None if r is None else r.data_ptr(), dy.data_ptr()
+    a.mean, a.rstd = _side(what, "mean", mean, (a.B, a.T), torch.float32, dev), _side(what, "rstd", rstd, (a.B, a.T), torch.float32, dev)
+    dr = torch.empty(x.shape, device=dev, dtype=x.dtype) if r is not None or not a.seed else None
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if a.seed else dr
+    a.dr, a.dx = None if dr is None else dr.data_ptr(), dx.data_ptr() if a.seed else None
+    a.dgamma, a.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
+    n = lib().svc_dropout_add_layernorm_ws_bytes(a.B, a.C, a.T)
+    ws = torch.empty((n,), device=dev, dtype=torch.uint8)
+    a.ws, a.ws_bytes = ws.data_ptr(), n
+    _launch_on(dev, lib().svc_dropout_add_layernorm_bwd, a, what)
+    return dx, dr if r is not None else None, dgamma, dbeta
