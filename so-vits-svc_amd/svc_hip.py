@@ -2018,11 +2018,12 @@ _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 def _launch_on(dev, fn, args, what):
     """fn(args, stream) on `dev`'s current stream, whatever the current device is."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(C.byref(args), torch.cuda.current_stream().cuda_stream)
+    i = dev.index
+    if i == torch.cuda.current_device():
+        rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(i))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(C.byref(args), torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(i):
+            rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(i))
     if rc:
         check(rc, what)
 
