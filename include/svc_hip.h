@@ -758,10 +758,10 @@ int svc_cmag_bwd_f32(const float* re, const float* im, const float* mag, const f
  * Accumulation, softmax statistics and gradients of the bias are fp32 for every dtype; P and dS are rounded to dtype as operands.
  *
  * svc_attn_scored_fwd writes out and, when not NULL, lse [B,H,Tq] (log2 of the sum of exp2 of the scores in log2 units; 0 for a query
- * without keys) and out32 [B,H*dk,Tq], contiguous: the output in fp32, for which P goes into the product as two operands of a 16-bit type
- * (its square's rounding instead of its own).  svc_attn_scored_bwd reads q, k, v, out32 (or out, when out32 is NULL), lse, dout and
- * writes dq, dk, dv (contiguous [B, heads*dk, T]) and dbias.  The rows' sums of dO out enter dbias unrounded, so 16-bit types' dbias, an fp32
- * result, wants out32.  No atomics on memory: results do not vary from run to run.  ws: svc_attn_scored_ws_bytes(a, backward) bytes, 16-byte aligned, contents undefined before and after.
+ * without keys) and out32 [B,H*dk,Tq], contiguous: the output in fp32, from which 16-bit types' backward takes its row sums of dO out.
+ * svc_attn_scored_bwd reads q, k, v, out32 (fp32: out), lse, dout and writes dq, dk, dv (contiguous [B, heads*dk, T]) and dbias.  The row sums enter
+ * dbias, an fp32 result of any type's call, unrounded: a forward whose dbias will be wanted is asked for with `exact`.  No atomics on memory:
+ * results do not vary from run to run.  scale > 0.  ws: svc_attn_scored_ws_bytes(a, backward) bytes, 16-byte aligned, contents undefined before and after.
  * Built for 1 <= dk <= 128, 0 <= Tq <= Tk < 2^30.
  * ---------------------------------------------------------------------------------------------- */
 enum { SVC_F32 = 0, SVC_BF16 = 1, SVC_F16 = 2 };
@@ -788,6 +788,7 @@ typedef struct svc_attn_scored_t {
   long long q_bs, q_cs, k_bs, k_cs, v_bs, v_cs, o_bs, o_cs, do_bs, do_cs;
   int dtype, B, H, G, dk, Tq, Tk;
   int causal, window, n_docs, offset, bias_w, bias_heads, site;
+  int exact;           /* 16-bit types: P as two (fp16) or three (bf16) operands and the library's tanh, what a fp32 dbias needs */
   float scale, softcap, p_drop;
 } svc_attn_scored_t;
 long long svc_attn_scored_ws_bytes(const svc_attn_scored_t* a, int backward);

@@ -86,6 +86,11 @@ __device__ __forceinline__ unsigned long long draw_word(unsigned long long start
   z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
   return z ^ (z >> 31);
 }
+// draw j of a word falls under the threshold (the odd fields compare in place, the even ones shifted up)
+__device__ __forceinline__ bool dropped(unsigned long long z, int j, unsigned thr) {
+  const unsigned w = (unsigned)(z >> (32 * (j >> 1)));
+  return (j & 1 ? w : w << 16) < thr << 16;
+}
 __device__ __forceinline__ unsigned long long draw_start(const svc_attn_scored_t& a) {
   return (unsigned long long)a.seed[0] + (unsigned long long)((unsigned)a.site + 1u) * 0x9E3779B97F4A7C15ull;
 }
@@ -111,62 +116,128 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __
 __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 
-// The columns t0 .. t0+31 of X[d][t] as a right operand that reduces over d (lane: column, half: d's second half of a step).
+// ---- staging: rows 0..DP-1 of X[d][p0 .. p0+N) into LDS rows of PITCH bytes, zero outside [beg, end) and behind row dk, so what lies there (unwritten
+// cache, padding) never reaches a product.  Rows may start at any alignment of their type.  In two halves, so that a tile's loads are in flight
+// while the one before is worked on: `fetch` into registers, `commit` to LDS.  A workgroup is 256 threads: 8 lanes a row, 32 rows a step.
+template <typename E, int DP> struct Pre { uint4 v[DP / 32]; };
+
 template <typename E, int DP>
-__device__ __forceinline__ void load_columns(typename Frag<E>::template Head<DP>& f, const E* x, long long cs, int dk, int t, int T, int h) {
-  const bool ok = t >= 0 && t < T;
-  if constexpr (sizeof(E) == 4) {
+struct Source {                         // one head's matrix as this thread sees it
+  const E *row, *last;                  // its row of step 0 and of the last step (whose rows may lie behind dk: the nearest row stands for them)
+  long long step;                       // elements between steps
+  int T;                                // positions that exist
+  bool pad;                             // its last row lies behind dk
+  __device__ __forceinline__ void set(const E* x, long long cs, int dk, int T_, int tid) {
+    const int d = tid >> 3, c = (tid & 7) * Tile<E>::V, dl = d + DP - 32;
+    row = x + (long long)d * cs + c;
+    last = x + (long long)min(dl, dk - 1) * cs + c;
+    step = 32 * cs;
+    T = T_;
+    pad = dl >= dk;
+    if (DP == 32) row = last;
+  }
+  __device__ __forceinline__ void fetch(Pre<E, DP>& f, int p0, int tid) const {
+    constexpr int S = DP / 32, V = Tile<E>::V;
+    if (p0 >= 0 && p0 + Tile<E>::N <= T) {
 #pragma unroll
-    for (int i = 0; i < DP / 2; ++i) {
-      const int d = 2 * i + h;
-      f.v[i] = ok && d < dk ? x[d * cs + t] : 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = 16 * i + 8 * h + e;
-        f.v[i][e] = ok && d < dk ? x[d * cs + t] : (E)0.f;
+      for (int i = 0; i < S; ++i) {
+        const U128 u = *(const U128*)((i == S - 1 ? last : row + i * step) + p0);
+        f.v[i] = make_uint4(u.x, u.y, u.z, u.w);
       }
-  }
-}
-
-// ---- staging: rows 0..DP-1 of X[d][p0 .. p0+N) into LDS rows of PITCH bytes; zero outside [beg, end) and behind row dk, so what
-// lies there (unwritten cache, padding) never reaches a product.  Rows may start at any alignment of their type.
-template <typename E>
-__device__ __forceinline__ uint4 load_chunk(const E* row, int p, int beg, int end) {
-  constexpr int V = Tile<E>::V;
-  if (p >= beg && p + V <= end) {
-    const U128 u = *(const U128*)(row + p);
-    return make_uint4(u.x, u.y, u.z, u.w);
-  }
-  union { uint4 u; E e[V]; } r;
-  r.u = make_uint4(0, 0, 0, 0);
+    } else {                            // the tile at the tensor's end: whole chunks as above, the one across the end by elements
+      const int p = p0 + (tid & 7) * V;
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (p + i >= beg && p + i < end) r.e[i] = row[p + i];
-  return r.u;
-}
-template <typename E, int DP>
-__device__ __forceinline__ void stage(E* lds, const E* x, long long cs, int dk, int p0, int beg, int end, int tid) {
+      for (int i = 0; i < S; ++i) {
+        const E* r = (i == S - 1 ? last : row + i * step) + p0;
+        union { uint4 u; E e[V]; } x;
+        x.u = make_uint4(0, 0, 0, 0);
+        if (p >= 0 && p + V <= T) {
+          const U128 u = *(const U128*)r;
+          x.u = make_uint4(u.x, u.y, u.z, u.w);
+        } else {
 #pragma unroll
-  for (int i = 0; i < DP * 8 / 256; ++i) {
-    const int idx = tid + 256 * i, d = idx >> 3, c = idx & 7;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (d < dk) v = load_chunk<E>(x + d * cs, p0 + c * Tile<E>::V, beg, end);
-    *(uint4*)((char*)lds + d * PITCH + c * 16) = v;
+          for (int e = 0; e < V; ++e)
+            if (p + e >= 0 && p + e < T) x.e[e] = r[e];
+        }
+        f.v[i] = x.u;
+      }
+    }
   }
-}
+  __device__ __forceinline__ void commit(E* lds, Pre<E, DP>& f, int p0, int beg, int end, int tid) const {
+    constexpr int S = DP / 32, V = Tile<E>::V;
+    if (p0 < beg || p0 + Tile<E>::N > end) {
+      const int p = p0 + (tid & 7) * V;
+      unsigned k[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(E) == 4) k[j] = p + j >= beg && p + j < end ? ~0u : 0u;
+        else k[j] = (p + 2 * j >= beg && p + 2 * j < end ? 0xffffu : 0u) | (p + 2 * j + 1 >= beg && p + 2 * j + 1 < end ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < S; ++i) f.v[i] = make_uint4(f.v[i].x & k[0], f.v[i].y & k[1], f.v[i].z & k[2], f.v[i].w & k[3]);
+    }
+    if (pad) f.v[S - 1] = make_uint4(0, 0, 0, 0);
+    char* o = (char*)lds + (tid >> 3) * PITCH + (tid & 7) * 16;
+#pragma unroll
+    for (int i = 0; i < S; ++i) *(uint4*)(o + i * 32 * PITCH) = f.v[i];
+  }
+};
 
-// acc[row = position, column] += sum_d X[d][position] * f[d][column]: rows = positions 32 rt .. 32 rt + 31 of the staged tile
+// Columns 32 sub .. 32 sub + 31 of a staged tile as a right operand that reduces over d.
 template <typename E, int DP>
-__device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typename Frag<E>::template Head<DP>& f, f32x16 acc, int lane) {
+__device__ __forceinline__ void read_columns(typename Frag<E>::template Head<DP>& f, const E* lds, int sub, int lane) {
   const int h = lane >> 5;
   if constexpr (sizeof(E) == 4) {
-    const float* p = lds + h * Tile<E>::P + 32 * rt + swap23(lane & 31);
+    const float* p = lds + h * Tile<E>::P + 32 * sub + (lane & 31);
 #pragma unroll
-    for (int i = 0; i < DP / 2; ++i) acc = mfma(p[2 * i * Tile<E>::P], f.v[i], acc);
+    for (int i = 0; i < DP / 2; ++i) f.v[i] = p[2 * i * Tile<E>::P];
+  } else {
+    const int i16 = lane & 15;
+    const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E>::P + 32 * sub + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      typedef __attribute__((address_space(3))) s16x4 lds4;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * i * Tile<E>::P));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + (16 * i + 4) * Tile<E>::P));
+      f.v[i] = __builtin_bit_cast(typename Frag<E>::V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+}
+
+// A workgroup's 128 columns of X as right operands, through the LDS of four tiles (16-bit types need two); [beg, end): columns that are used.
+template <typename E, int DP>
+__device__ __forceinline__ void load_columns(typename Frag<E>::template Head<DP>& f, E* lds, const E* x, long long cs, int dk, int T, int t0, int beg, int end,
+                                             int tid) {
+  constexpr int N = Tile<E>::N;
+  Source<E, DP> src;
+  src.set(x, cs, dk, T, tid);
+  Pre<E, DP> pre[NCOL / N];
+#pragma unroll
+  for (int i = 0; i < NCOL / N; ++i) src.fetch(pre[i], t0 + i * N, tid);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NCOL / N; ++i) src.commit(lds + i * DP * Tile<E>::P, pre[i], t0 + i * N, beg, end, tid);
+  __syncthreads();
+  const int col = (tid >> 6) * 32;
+  read_columns<E, DP>(f, lds + col / N * DP * Tile<E>::P, col % N / 32, tid & 63);
+}
+
+// -> [row = position, column]: sum_d X[d][position] * f[d][column]: rows = positions 32 rt .. 32 rt + 31 of the staged tile
+template <typename E, int DP>
+__device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typename Frag<E>::template Head<DP>& f, int lane) {
+  const int h = lane >> 5;
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  if constexpr (sizeof(E) == 4) {
+    // four sums of a quarter of the channels each: a chain's rounding errors grow with its length and with the sums it passes through
+    const float* p = lds + h * Tile<E>::P + 32 * rt + swap23(lane & 31);
+    f32x16 part[4] = {acc, acc, acc, acc};
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[j] = mfma(p[2 * (j * (DP / 8) + i) * Tile<E>::P], f.v[j * (DP / 8) + i], part[j]);
+    acc = (part[0] + part[1]) + (part[2] + part[3]);
   } else {
     const int i16 = lane & 15, c = i16 & 3;
     const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E>::P + 32 * rt + 16 * ((lane >> 4) & 1) + 4 * (((c & 1) << 1) | (c >> 1));
@@ -183,8 +254,8 @@ __device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typena
 }
 
 // out[d, column] += sum_position X[d][position] * w[position, column], w in accumulator layout (rows 32 rt .. of the tile).  16-bit types round w
-// to the type; TWO: w goes in as two operands, its rounded value and the rounded rest (u^2 instead of u).
-template <typename E, int DP, bool TWO = false>
+// to the type; OPS > 1: w goes in as that many operands, its rounded value, the rounded rest, and the rest of that.
+template <typename E, int DP, int OPS = 1>
 __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, int rt, const float (&w)[16], int lane) {
   const int h = lane >> 5;
   const E* p = lds + (lane & 31) * Tile<E>::P + 32 * rt + 8 * h;
@@ -200,38 +271,71 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
   } else {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      typename Frag<E>::V b, rest;
+      typename Frag<E>::V b[OPS];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        b[e] = (E)w[8 * ks + e];
-        if constexpr (TWO) rest[e] = (E)(w[8 * ks + e] - (float)b[e]);
+        float rest = w[8 * ks + e];
+#pragma unroll
+        for (int o = 0; o < OPS; ++o) {
+          b[o][e] = (E)rest;
+          rest -= (float)b[o][e];
+        }
       }
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
         const typename Frag<E>::V v = *(const typename Frag<E>::V*)(p + 32 * dt * Tile<E>::P + 16 * ks);
-        out[dt] = mfma(v, b, out[dt]);
-        if constexpr (TWO) out[dt] = mfma(v, rest, out[dt]);
+#pragma unroll
+        for (int o = 0; o < OPS; ++o) out[dt] = mfma(v, b[o], out[dt]);
       }
     }
   }
 }
 
-// ---- scores in units of log 2: u = cap * tanh(scale q.k / cap) or scale q.k, times log2(e), plus the (already scaled) bias --------
+// ---- scores in units of log 2 ------------------------------------------------------------------------------------------------------------
 struct ScoreScale {
-  float mul, cap_in, cap_out;      // mul: no cap; else tanh(acc * cap_in) * cap_out
+  float mul, cap_in, cap_out;      // no cap: u * mul; else tanh(u * cap_in) * cap_out
+  bool cap;
 };
 __device__ __forceinline__ ScoreScale score_scale(const svc_attn_scored_t& a) {
   ScoreScale s;
+  s.cap = a.softcap > 0.f;
   s.mul = a.scale * LOG2E;
-  s.cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  s.cap_in = s.cap ? a.scale / a.softcap : 0.f;
   s.cap_out = a.softcap * LOG2E;
   return s;
 }
+// tanh for the cap.  EXACT (fp32, and where a fp32 gradient of the bias hangs on it): the library's.  Else 1 - 2 / (exp 2x + 1), two
+// transcendental instructions: 1e-7 absolute, so 1e-7 of the cap in a score whose P and result are rounded to 2^-8 or 2^-11.
+template <bool EXACT> __device__ __forceinline__ float cap_tanh(float x) {
+  if (EXACT) return tanhf(x);
+  return fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * LOG2E)) + 1.f), 1.f);
+}
 
-// The distance bias of a tile: win[j] = table[clamp(d0 + j, -W, W) + W] * log2(e) for j in [0, n): the tile's distances are
-// consecutive, so the table's clamped entries become one short row in LDS and a lookup an offset from a lane's own base.
-__device__ __forceinline__ void stage_bias(float* win, const float* table, int W, int d0, int n, int tid) {
-  for (int j = tid; j < n; j += 256) win[j] = table[min(max(d0 + j, -W), W) + W] * LOG2E;
+// The distance bias of a tile: win[j] = table[clamp(d0 + j, -W, W) + W] * log2(e) for j in [0, n), n <= 256: the tile's distances are consecutive, so the
+// table's clamped entries become one short row in LDS and a lookup an offset from a lane's own base.  Thread j fetches and commits entry j.
+__device__ __forceinline__ float bias_entry(const float* table, int W, int d0, int j) { return table[min(max(d0 + j, -W), W) + W] * LOG2E; }
+
+// ---- which (item, head, tile) a workgroup works on.  Tiles from the heaviest on (the last, under a causal mask), all heads of one tile index before the
+// next; where the key heads divide by the 8 XCDs (or there are so many that it hardly matters), a key head's workgroups share one XCD and its L2.
+struct Place { int group, sub, tile; };           // group = item * G + key head; sub: query head of the group
+__host__ __device__ __forceinline__ bool by_xcd(int groups) { return groups % 8 == 0 || groups >= 64; }
+__device__ __forceinline__ Place place_of(int id, int groups, int rep, int n_tiles) {
+  Place p;
+  if (by_xcd(groups)) {
+    const int per = (groups + 7) / 8 * rep, j = id >> 3, r = j % per;
+    p.tile = n_tiles - 1 - j / per;
+    p.group = r / rep * 8 + (id & 7);
+    p.sub = r % rep;
+  } else {
+    const int r = id % (groups * rep);
+    p.tile = n_tiles - 1 - id / (groups * rep);
+    p.group = r / rep;
+    p.sub = r % rep;
+  }
+  return p;
+}
+static inline long long grid_of(long long groups, long long rep, long long n_tiles) {
+  return (by_xcd((int)groups) ? (groups + 7) / 8 * 8 : groups) * rep * n_tiles;
 }
 
 __device__ __forceinline__ int wave_min(int v) {
@@ -244,5 +348,36 @@ __device__ __forceinline__ int wave_max(int v) {
 }
 
 int check_args(const svc_attn_scored_t* a, bool backward);      // attn_scored_fwd.hip
+
+// ---- the backward's workspace -----------------------------------------------------------------------------------------------------------
+struct Ws {
+  float* rowsum;   // [B*H][Tq]  D = sum_d dO out
+  int2* iv;        // [B][Tq]    visible keys
+  int4* tiles;     // [B][ceil(Tq/32)]  {min lo, max hi, max lo, min hi} of 32 queries
+  float* gmax;     // [B*H][ceil(Tq/64)]  max |dO|
+  float* bins;     // [B*H][ceil(Tq/32)][2 bias_w + 1]  bias gradient of 32 queries
+  long long bytes;
+};
+void launch_dq(const svc_attn_scored_t& a, const Ws& w, hipStream_t s);        // attn_scored_dq.hip
+void launch_dkv(const svc_attn_scored_t& a, const Ws& w, hipStream_t s);       // attn_scored_dkv.hip
+
+// fp16 operands: dS is multiplied by a power of two that brings the largest |dO| of the key head to [1, 2): gradients of any magnitude then
+// sit in the middle of the type's range (a loss scale of 2^-12 would otherwise leave dS among its subnormals), and |dS| <= 2 P |dO| |v|
+// dk stays below 65504 for |v| up to 250.  The factor is divided out of the fp32 accumulators.
+template <typename E> __device__ __forceinline__ float operand_scale(const svc_attn_scored_t& a, const Ws& w, int b, int kvh, float* red) {
+  if constexpr (!__is_same(E, f16_t)) return 1.f;
+  const int n_tiles = (a.Tq + 63) / 64, rep = a.H / a.G, n = rep * n_tiles;
+  const float* g = w.gmax + ((long long)b * a.H + (long long)kvh * rep) * n_tiles;
+  float m = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) m = fmaxf(m, g[i]);
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (!(m > 0.f) || !(m < INFINITY)) return 1.f;
+  int e;
+  frexpf(m, &e);
+  return ldexpf(1.f, 1 - e);
+}
 
 }  // namespace attn

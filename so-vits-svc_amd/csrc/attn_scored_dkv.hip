@@ -1,0 +1,226 @@
+// attn_scored_dkv.hip — svc_attn_scored_bwd's walk over the queries: dk and dv.
+#include "attn_scored.h"
+
+namespace attn {
+
+template <int J> __device__ __forceinline__ unsigned quad(unsigned v) {      // lane J of the own four
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)v, J * 0x55, 0xf, 0xf, true);
+}
+
+// 128 keys of one key head a workgroup (32 a wave), walking the query tiles of its query heads that see any of them.
+template <typename E, int DP, bool EXACT>
+__global__ __launch_bounds__(256, 2) void dkv_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
+  constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
+  __shared__ __align__(16) char tiles_[4 * DP * PITCH];
+  __shared__ float win[2][NCOL + N];
+  __shared__ __align__(16) float lses[2][N], rows[2][N];
+  __shared__ __align__(16) int2 ivs[2][N];
+  __shared__ float red[4];
+  E* const tiles = (E*)tiles_;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, n = lane & 31, rep = a.H / a.G;
+  const Place at = place_of(blockIdx.x, a.B * a.G, 1, n_tiles);
+  if (at.group >= a.B * a.G) return;
+  // (under a causal mask the first keys are the heaviest)
+  const int bg = at.group, c0 = (n_tiles - 1 - at.tile) * NCOL, b = bg / a.G, kvh = bg % a.G;
+  const int w0 = c0 + wave * 32, sl = wave * 32 + n, s = c0 + sl;
+  const int off = item_offset(a, b), len = item_length(a, b);
+  const float g2 = operand_scale<E>(a, ws, b, kvh, red), pup = exp2f(PUP<E>), gm = g2 / pup;
+  // queries that can see a key at all, and keys that can be seen: what lies in the others' columns is not used
+  const int o1 = min(max(off, -a.Tq), a.Tk);
+  int tbeg = max(0, -o1), tend = max(0, min(a.Tq, len - o1)), kbeg = 0, kend = len;
+  if (a.n_docs) {
+    const int* d = a.docs + (long long)b * (a.n_docs + 1);
+    kbeg = max(0, d[0]);
+    kend = max(0, min(len, d[a.n_docs]));
+    tbeg = max(tbeg, kbeg - o1);
+    tend = min(tend, kend - o1);
+  }
+  typename Frag<E>::template Head<DP> k, v;
+  load_columns<E, DP>(k, tiles, (const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, c0, kbeg, kend, tid);
+  load_columns<E, DP>(v, tiles, (const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, c0, kbeg, kend, tid);
+  const ScoreScale sc = score_scale(a);
+  unsigned thr = 0;
+  float keep = 1.f;
+  unsigned long long start = 0;
+  const unsigned long long ng = (unsigned long long)((a.Tk + 3) >> 2);
+  if (a.seed) {
+    start = draw_start(a) + (unsigned)(s >> 2) * 0xD1B54A32D192ED03ull;
+    thr = (unsigned)rintf(a.p_drop * 65536.f);
+    keep = 65536.f / (65536.f - (float)thr);
+  }
+  f32x16 ak[DP / 32], av[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ak[i][r] = av[i][r] = 0.f;
+
+  // The walk: (query head, tile) pairs whose tile has a query that sees a key of the workgroup's.
+  const int t32 = (a.Tq + 31) / 32;
+  const int4* const spans = ws.tiles + (long long)b * t32;
+  auto span = [&](int t0) {
+    int4 r = spans[t0 >> 5];
+    if (RT == 2 && t0 + 32 < a.Tq) {
+      const int4 r1 = spans[(t0 >> 5) + 1];
+      r = make_int4(min(r.x, r1.x), max(r.y, r1.y), max(r.z, r1.z), min(r.w, r1.w));
+    }
+    return r;
+  };
+  auto advance = [&](int& hh, int& t0, int4& r) {            // to the first pair from (hh, t0) on; hh = rep: none
+    for (; hh < rep; ++hh, t0 = 0)
+      for (; t0 < a.Tq; t0 += N) {
+        r = span(t0);
+        if (r.x < c0 + NCOL && r.y > c0) return;
+      }
+  };
+  Source<E, DP> qsrc, gsrc;
+  Pre<E, DP> qf, gf;
+  float bf = 0.f, lf = 0.f, rf = 0.f;
+  int2 vf = make_int2(0, 0);
+  auto fetch = [&](int hh, int t0) {
+    const int head = kvh * rep + hh;
+    const long long bh = (long long)b * a.H + head;
+    qsrc.set((const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs, a.q_cs, a.dk, a.Tq, tid);
+    gsrc.set((const E*)a.dout + b * a.do_bs + (long long)head * a.dk * a.do_cs, a.do_cs, a.dk, a.Tq, tid);
+    qsrc.fetch(qf, t0, tid);
+    gsrc.fetch(gf, t0, tid);
+    if (a.bias && tid < NCOL + N)
+      bf = bias_entry(a.bias + (a.bias_heads > 1 ? (long long)head * (2 * a.bias_w + 1) : 0), a.bias_w, c0 - (off + t0) - (N - 1), tid);
+    if (tid < N) {
+      const int t = t0 + tid;
+      const bool in = t < a.Tq;
+      lf = in ? a.lse[bh * a.Tq + t] - PUP<E> : 0.f;
+      rf = in ? ws.rowsum[bh * a.Tq + t] : 0.f;
+      vf = in ? ws.iv[(long long)b * a.Tq + t] : make_int2(0, 0);
+    }
+  };
+  int hh = 0, t0 = 0, buf = 0;
+  int4 r = make_int4(0, 0, 0, 0);
+  advance(hh, t0, r);
+  if (hh < rep) fetch(hh, t0);
+  __syncthreads();                                           // (the keys' columns have been read from the tiles)
+  while (hh < rep) {
+    E* const qs = tiles + buf * 2 * DP * Tile<E>::P;
+    E* const gs = qs + DP * Tile<E>::P;
+    qsrc.commit(qs, qf, t0, tbeg, tend, tid);
+    gsrc.commit(gs, gf, t0, tbeg, tend, tid);
+    if (a.bias && tid < NCOL + N) win[buf][tid] = bf;
+    if (tid < N) {
+      lses[buf][tid] = lf;
+      rows[buf][tid] = rf;
+      ivs[buf][tid] = vf;
+    }
+    __syncthreads();
+    const int head = kvh * rep + hh, now = t0;
+    const bool work = r.x < w0 + 32 && r.y > w0, whole = w0 >= r.z && w0 + 32 <= r.w && now + N <= a.Tq;
+    t0 += N;
+    advance(hh, t0, r);
+    if (hh < rep) fetch(hh, t0);
+    const int cur = buf;
+    buf ^= 1;
+    if (!work) continue;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const f32x16 u = mul_columns<E, DP>(qs, rt, k, lane);
+      f32x16 dp = mul_columns<E, DP>(gs, rt, v, lane);
+      float x[16], th[16], p[16], mul = sc.mul;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = u[i];
+      if (sc.cap) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          th[i] = cap_tanh<EXACT>(x[i] * sc.cap_in);
+          x[i] = th[i] * sc.cap_out;
+        }
+        mul = 1.f;
+      }
+      if (a.bias) {
+        const float* w = win[cur] + (N - 1) - 32 * rt + sl;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = fmaf(x[i], mul, w[-pos_of(i, h)]);
+        mul = 1.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], mul, -lses[cur][32 * rt + pos_of(i, h)]));
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int2 w = ivs[cur][32 * rt + pos_of(i, h)];
+          x[i] = s >= w.x && s < w.y ? x[i] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = x[i];
+      if (a.seed) {
+        // A word holds the draws of four neighbouring keys, which are four neighbouring lanes: lane j of the four works out the word of row 4w + j and
+        // all of them read it from there.
+        const unsigned long long row = (unsigned long long)(((long long)b * a.H + head) * a.Tq + now + 32 * rt);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const unsigned long long z = draw_word(start, (row + pos_of(4 * w, h) + (n & 3)) * ng);
+          const unsigned lo = (unsigned)z, hi = (unsigned)(z >> 32);
+          auto one = [&](int i, unsigned l, unsigned g) {
+            const unsigned f = n & 2 ? g : l;
+            const bool drop = (n & 1 ? f : f << 16) < thr << 16;
+            p[i] = drop ? 0.f : x[i] * keep;
+            dp[i] = drop ? 0.f : dp[i] * keep;
+          };
+          one(4 * w, quad<0>(lo), quad<0>(hi));
+          one(4 * w + 1, quad<1>(lo), quad<1>(hi));
+          one(4 * w + 2, quad<2>(lo), quad<2>(hi));
+          one(4 * w + 3, quad<3>(lo), quad<3>(hi));
+        }
+      }
+      mul_rows<E, DP>(av, gs, rt, p, lane);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float g = x[i] * (dp[i] - rows[cur][32 * rt + pos_of(i, h)]);
+        x[i] = whole || x[i] > 0.f ? g : 0.f;                // (a masked entry: 0 whatever dO.v is)
+      }
+      if (sc.cap) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
+      }
+      if constexpr (__is_same(E, f16_t)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= gm;
+      }
+      mul_rows<E, DP>(ak, qs, rt, x, lane);
+    }
+  }
+  if (s >= a.Tk) return;
+  const float os = a.scale / g2, ov = 1.f / pup;
+  E* dk = (E*)a.dk_ + (long long)bg * a.dk * a.Tk + s;
+  E* dv = (E*)a.dv + (long long)bg * a.dk * a.Tk + s;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int d = 32 * i + 8 * (j >> 2) + 4 * h + (j & 3);
+      if (d < a.dk) {
+        dk[(long long)d * a.Tk] = (E)(ak[i][j] * os);
+        dv[(long long)d * a.Tk] = (E)(av[i][j] * ov);
+      }
+    }
+}
+
+template <typename E, int DP>
+static void go(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
+  const int n_tiles = (a.Tk + NCOL - 1) / NCOL;
+  const unsigned grid = (unsigned)grid_of((long long)a.B * a.G, 1, n_tiles);
+  if (sizeof(E) == 4 || a.dbias) hipLaunchKernelGGL((dkv_kernel<E, DP, true>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
+  else hipLaunchKernelGGL((dkv_kernel<E, DP, sizeof(E) == 4>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
+}
+template <typename E>
+static void pick(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
+  if (a.dk <= 32) go<E, 32>(a, w, s);
+  else if (a.dk <= 64) go<E, 64>(a, w, s);
+  else if (a.dk <= 96) go<E, 96>(a, w, s);
+  else go<E, 128>(a, w, s);
+}
+void launch_dkv(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
+  if (a.dtype == SVC_F32) pick<float>(a, w, s);
+  else if (a.dtype == SVC_BF16) pick<bf16_t>(a, w, s);
+  else pick<f16_t>(a, w, s);
+}
+
+}  // namespace attn

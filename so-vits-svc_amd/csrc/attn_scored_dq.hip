@@ -1,0 +1,239 @@
+// attn_scored_dq.hip — svc_attn_scored_bwd's walk over the keys: dq and the bias gradient.
+#include "attn_scored.h"
+
+namespace attn {
+
+// 128 queries of one head a workgroup (32 a wave), walking the key tiles that any of them sees.
+template <typename E, int DP, bool EXACT>
+__global__ __launch_bounds__(256, 2) void dq_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
+  constexpr int N = Tile<E>::N, RT = Tile<E>::RT, NB = N + 32;
+  __shared__ __align__(16) char tiles_[4 * DP * PITCH];
+  __shared__ float win[2][NCOL + N];
+  __shared__ float bin_[4][2][NB];
+  __shared__ int range[2][4];
+  __shared__ float red[4];
+  E* const tiles = (E*)tiles_;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, n = lane & 31;
+  const Place at = place_of(blockIdx.x, a.B * a.G, a.H / a.G, n_tiles);
+  if (at.group >= a.B * a.G) return;
+  const int b = at.group / a.G, kvh = at.group % a.G, head = kvh * (a.H / a.G) + at.sub, t0 = at.tile * NCOL;
+  const long long bh = (long long)b * a.H + head;
+
+  const int tl = wave * 32 + n, t = t0 + tl;
+  const int off = item_offset(a, b);
+  const int2 iv = t < a.Tq ? ws.iv[(long long)b * a.Tq + t] : make_int2(0, 0);
+  const bool some = iv.y > iv.x;
+  const int wlo = wave_min(some ? iv.x : a.Tk), whi = wave_max(iv.y);
+  const int flo = wave_max(t < a.Tq ? (some ? iv.x : a.Tk) : 0), fhi = wave_min(t < a.Tq ? iv.y : a.Tk);
+  const int clo = wave_min(some ? t : a.Tq), chi = wave_max(some ? t + 1 : 0);
+  __shared__ int cols[2][4];
+  if (lane == 0) {
+    range[0][wave] = wlo;
+    range[1][wave] = whi;
+    cols[0][wave] = clo;
+    cols[1][wave] = chi;
+  }
+  const float gs = operand_scale<E>(a, ws, b, kvh, red);
+  __syncthreads();
+  const int blo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3]));
+  const int bhi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
+  // what q and dO hold before the first and behind the last query that sees anything is not used
+  const int cbeg = min(min(cols[0][0], cols[0][1]), min(cols[0][2], cols[0][3])), cend = max(max(cols[1][0], cols[1][1]), max(cols[1][2], cols[1][3]));
+
+  typename Frag<E>::template Head<DP> q, g;
+  load_columns<E, DP>(q, tiles, (const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs, a.q_cs, a.dk, a.Tq, t0, cbeg, cend, tid);
+  load_columns<E, DP>(g, tiles, (const E*)a.dout + b * a.do_bs + (long long)head * a.dk * a.do_cs, a.do_cs, a.dk, a.Tq, t0, cbeg, cend, tid);
+  const float lse = some ? a.lse[bh * a.Tq + t] : 0.f, D = some ? ws.rowsum[bh * a.Tq + t] : 0.f;
+  const ScoreScale sc = score_scale(a);
+  const float* table = a.bias ? a.bias + (a.bias_heads > 1 ? (long long)head * (2 * a.bias_w + 1) : 0) : nullptr;
+  const int d0 = -(off + t0) - (NCOL - 1);
+  unsigned long long draws = 0;
+  unsigned thr = 0;
+  float keep = 1.f;
+  if (a.seed) {
+    draws = draw_start(a) + (unsigned long long)(bh * a.Tq + t) * (unsigned long long)((a.Tk + 3) >> 2) * 0xD1B54A32D192ED03ull;
+    thr = (unsigned)rintf(a.p_drop * 65536.f);
+    keep = 65536.f / (65536.f - (float)thr);
+  }
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+
+  // Bias gradient.  The tile's entries of one distance lie on a diagonal: lane n of half h adds register r to bin pos(r,h) - n + 31 of its
+  // half's own row, so the lanes of one instruction never meet (a half has 32 different n) and neither do waves: LDS adds in a fixed order.
+  // As the tiles advance by N keys, a wave's first N bins are complete after each tile and leave; the last 32 stay.  Distances at or
+  // beyond +-bias_w share the table's end entries and are summed in registers.
+  const int W = a.bias_w;
+  float* const bin = bin_[wave][h];
+  float* bins = a.dbias ? ws.bins + (bh * ((a.Tq + 31) / 32) + (t0 >> 5) + wave) * (2 * W + 1) : nullptr;
+  float end_lo = 0.f, end_hi = 0.f;
+  const int p31 = off + t0 + wave * 32 + 31;               // the wave's last query position: bin j of a tile at s0 is distance s0 - p31 + j
+  const bool live = a.dbias && (t0 >> 5) + wave < (a.Tq + 31) / 32;
+  int first_d = 0, base = 0;                               // distances of the first bin ever and of bin 0 now
+  bool begun = false;
+  if (a.dbias)
+    for (int j = n; j < NB; j += 32) bin[j] = 0.f;
+
+  Source<E, DP> ksrc, vsrc;
+  ksrc.set((const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, tid);
+  vsrc.set((const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, tid);
+  Pre<E, DP> kf, vf;
+  float bf = 0.f;
+  const int first = blo / N * N;
+  if (first < bhi) {
+    ksrc.fetch(kf, first, tid);
+    vsrc.fetch(vf, first, tid);
+    if (table && tid < NCOL + N) bf = bias_entry(table, W, first + d0, tid);
+  }
+  int buf = 0;
+  for (int s0 = first; s0 < bhi; s0 += N, buf ^= 1) {
+    E* const ks = tiles + buf * 2 * DP * Tile<E>::P;
+    E* const vs = ks + DP * Tile<E>::P;
+    if (s0 == first) __syncthreads();
+    ksrc.commit(ks, kf, s0, blo, bhi, tid);
+    vsrc.commit(vs, vf, s0, blo, bhi, tid);
+    if (table && tid < NCOL + N) win[buf][tid] = bf;
+    __syncthreads();
+    if (s0 + N < bhi) {
+      ksrc.fetch(kf, s0 + N, tid);
+      vsrc.fetch(vf, s0 + N, tid);
+      if (table && tid < NCOL + N) bf = bias_entry(table, W, s0 + N + d0, tid);
+    }
+    if (s0 >= whi || s0 + N <= wlo) continue;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const f32x16 u = mul_columns<E, DP>(ks, rt, q, lane);
+      f32x16 dp = mul_columns<E, DP>(vs, rt, g, lane);
+      float x[16], th[16];
+      float mul = sc.mul;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = u[r];
+      if (sc.cap) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          th[r] = cap_tanh<EXACT>(x[r] * sc.cap_in);
+          x[r] = th[r] * sc.cap_out;
+        }
+        mul = 1.f;
+      }
+      if (table) {
+        const float* w = win[buf] + 32 * rt + (NCOL - 1) - tl;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], mul, w[pos_of(r, h)]);
+        mul = 1.f;
+      }
+      if (a.seed) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const unsigned long long z = draw_word(draws, (unsigned long long)((s0 + 32 * rt + pos_of(4 * w, h)) >> 2));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dp[4 * w + j] = dropped(z, j, thr) ? 0.f : dp[4 * w + j] * keep;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, -lse)) * (dp[r] - D);
+      if (s0 < flo || s0 + N > fhi) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const unsigned p = s0 + 32 * rt + pos_of(r, h) - iv.x;
+          x[r] = p < (unsigned)(iv.y - iv.x) ? x[r] : 0.f;
+        }
+      }
+      if (a.dbias) {
+        const int d_lo = s0 + 32 * rt - p31, d_hi = d_lo + 62;      // the 32 x 32 block's distances
+        if (d_hi <= -W) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) end_lo += x[r];
+        } else if (d_lo >= W) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) end_hi += x[r];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(&bin[32 * rt + pos_of(r, h) - n + 31], x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        }
+      }
+      if (sc.cap) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] *= fmaf(-th[r], th[r], 1.f);
+      }
+      if constexpr (__is_same(E, f16_t)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] *= gs;
+      }
+      mul_rows<E, DP>(acc, ks, rt, x, lane);
+    }
+    if (live) {
+      // N complete bins leave (N = 64: one a lane; N = 32: the lower half of the lanes), 32 stay
+      if (!begun) first_d = s0 - p31;
+      begun = true;
+      base = s0 - p31 + N;
+      if (s0 + N - 1 - p31 + 31 > -W && s0 - p31 < W) {     // (else the tile and what stayed are past the ends: nothing was added to bins that leave)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const float v = lane < N ? bin_[wave][0][lane] + bin_[wave][1][lane] : 0.f;
+        const float stay = bin[N + n];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int j = n; j < NB; j += 32) bin[j] = j < 32 ? stay : 0.f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int d = s0 - p31 + lane;
+        if (lane < N) {
+          if (d <= -W) end_lo += v;
+          else if (d >= W) end_hi += v;
+          else bins[d + W] = v;
+        }
+      }
+    }
+  }
+  if (live) {
+    if (begun && lane < 32) {
+      const float v = bin_[wave][0][lane] + bin_[wave][1][lane];
+      const int d = base + lane;
+      if (d <= -W) end_lo += v;
+      else if (d >= W) end_hi += v;
+      else bins[d + W] = v;
+    }
+    for (int e = 1 - W + lane; e < W; e += 64)
+      if (!begun || e < first_d || e >= base + 32) bins[e + W] = 0.f;
+    for (int o = 32; o > 0; o >>= 1) {
+      end_lo += __shfl_xor(end_lo, o);
+      end_hi += __shfl_xor(end_hi, o);
+    }
+    if (lane == 0) {
+      bins[0] = W ? end_lo : end_lo + end_hi;
+      if (W) bins[2 * W] = end_hi;
+    }
+  }
+  if (t >= a.Tq) return;
+  const float os = a.scale / gs;
+  E* o = (E*)a.dq + bh * a.dk * a.Tq + t;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int d = 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
+      if (d < a.dk) o[(long long)d * a.Tq] = (E)(acc[i][r] * os);
+    }
+}
+
+template <typename E, int DP>
+static void go(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
+  const int n_tiles = (a.Tq + NCOL - 1) / NCOL;
+  const unsigned grid = (unsigned)grid_of((long long)a.B * a.G, a.H / a.G, n_tiles);
+  if (sizeof(E) == 4 || a.dbias) hipLaunchKernelGGL((dq_kernel<E, DP, true>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
+  else hipLaunchKernelGGL((dq_kernel<E, DP, sizeof(E) == 4>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
+}
+template <typename E>
+static void pick(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
+  if (a.dk <= 32) go<E, 32>(a, w, s);
+  else if (a.dk <= 64) go<E, 64>(a, w, s);
+  else if (a.dk <= 96) go<E, 96>(a, w, s);
+  else go<E, 128>(a, w, s);
+}
+void launch_dq(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
+  if (a.dtype == SVC_F32) pick<float>(a, w, s);
+  else if (a.dtype == SVC_BF16) pick<bf16_t>(a, w, s);
+  else pick<f16_t>(a, w, s);
+}
+
+}  // namespace attn

@@ -5,20 +5,20 @@
 namespace attn {
 
 // A workgroup owns 128 queries of one head (32 a wave) and walks the key tiles that any of them sees.
-template <typename E, int DP>
-__global__ __launch_bounds__(256) void fwd_kernel(svc_attn_scored_t a, int n_tiles) {
+template <typename E, int DP, bool EXACT>
+__global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_tiles) {
   constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
-  __shared__ __align__(16) char ks_[DP * PITCH], vs_[DP * PITCH];
-  __shared__ float win[NCOL + N];
+  // a maximum that grows by less than this (a factor 2^LAZY in P) leaves the accumulators as they are: P stays far from any type's range
+  constexpr float LAZY = __is_same(E, f16_t) ? 4.f : 8.f;
+  __shared__ __align__(16) char tiles_[4 * DP * PITCH];
+  __shared__ float win[2][NCOL + N];
   __shared__ int range[2][4];
-  E* ks = (E*)ks_;
-  E* vs = (E*)vs_;
+  E* const tiles = (E*)tiles_;                                    // [2 buffers][k, v][DP][P]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, n = lane & 31;
-  const int bh = blockIdx.x / n_tiles, t0 = (blockIdx.x % n_tiles) * NCOL;
-  const int b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.G);
-  const E* kp = (const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs;
-  const E* vp = (const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs;
-  const E* qp = (const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs;
+  const Place at = place_of(blockIdx.x, a.B * a.G, a.H / a.G, n_tiles);
+  if (at.group >= a.B * a.G) return;
+  const int b = at.group / a.G, kvh = at.group % a.G, head = kvh * (a.H / a.G) + at.sub, t0 = at.tile * NCOL;
+  const long long bh = (long long)b * a.H + head;
 
   const int tl = wave * 32 + n, t = t0 + tl;
   const int len = item_length(a, b), off = item_offset(a, b);
@@ -32,19 +32,18 @@ __global__ __launch_bounds__(256) void fwd_kernel(svc_attn_scored_t a, int n_til
     range[0][wave] = wlo;
     range[1][wave] = whi;
   }
-  __syncthreads();
+  typename Frag<E>::template Head<DP> q;
+  load_columns<E, DP>(q, tiles, (const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs, a.q_cs, a.dk, a.Tq, t0, 0, a.Tq, tid);
   const int blo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3]));
   const int bhi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
 
-  typename Frag<E>::template Head<DP> q;
-  load_columns<E, DP>(q, qp, a.q_cs, a.dk, t, a.Tq, h);
   const ScoreScale sc = score_scale(a);
   const float* table = a.bias ? a.bias + (a.bias_heads > 1 ? (long long)head * (2 * a.bias_w + 1) : 0) : nullptr;
+  const int d0 = -(off + t0) - (NCOL - 1);                        // distance of window entry 0 in a tile at key 0
   unsigned long long draws = 0;
   unsigned thr = 0;
   if (a.seed) {
-    const unsigned long long row = ((unsigned long long)b * a.H + head) * a.Tq + t;
-    draws = draw_start(a) + row * (unsigned long long)((a.Tk + 3) >> 2) * 0xD1B54A32D192ED03ull;
+    draws = draw_start(a) + (unsigned long long)(bh * a.Tq + t) * (unsigned long long)((a.Tk + 3) >> 2) * 0xD1B54A32D192ED03ull;
     thr = (unsigned)rintf(a.p_drop * 65536.f);
   }
   f32x16 acc[DP / 32];
@@ -54,70 +53,98 @@ __global__ __launch_bounds__(256) void fwd_kernel(svc_attn_scored_t a, int n_til
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  for (int s0 = blo / N * N; s0 < bhi; s0 += N) {
+  Source<E, DP> ksrc, vsrc;
+  ksrc.set((const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, tid);
+  vsrc.set((const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, tid);
+  Pre<E, DP> kf, vf;
+  float bf = 0.f;
+  const int first = blo / N * N;
+  if (first < bhi) {
+    ksrc.fetch(kf, first, tid);
+    vsrc.fetch(vf, first, tid);
+    if (table && tid < NCOL + N) bf = bias_entry(table, a.bias_w, first + d0, tid);
+  }
+  int buf = 0;
+  for (int s0 = first; s0 < bhi; s0 += N, buf ^= 1) {
+    E* const ks = tiles + buf * 2 * DP * Tile<E>::P;
+    E* const vs = ks + DP * Tile<E>::P;
+    if (s0 == first) __syncthreads();                             // (q's columns have been read from the tiles)
+    ksrc.commit(ks, kf, s0, blo, bhi, tid);
+    vsrc.commit(vs, vf, s0, blo, bhi, tid);
+    if (table && tid < NCOL + N) win[buf][tid] = bf;
     __syncthreads();
-    stage<E, DP>(ks, kp, a.k_cs, a.dk, s0, blo, bhi, tid);
-    stage<E, DP>(vs, vp, a.v_cs, a.dk, s0, blo, bhi, tid);
-    if (table) stage_bias(win, table, a.bias_w, s0 - (off + t0) - (NCOL - 1), NCOL + N, tid);
-    __syncthreads();
+    if (s0 + N < bhi) {
+      ksrc.fetch(kf, s0 + N, tid);
+      vsrc.fetch(vf, s0 + N, tid);
+      if (table && tid < NCOL + N) bf = bias_entry(table, a.bias_w, s0 + N + d0, tid);
+    }
     if (s0 >= whi || s0 + N <= wlo) continue;
     float s[RT][16];
-    float mt = -INFINITY;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      f32x16 u;
+      const f32x16 u = mul_columns<E, DP>(ks, rt, q, lane);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) u[r] = 0.f;
-      u = mul_columns<E, DP>(ks, rt, q, u, lane);
-      if (sc.cap_in > 0.f) {
+      for (int r = 0; r < 16; ++r) s[rt][r] = u[r];
+    }
+    float mul = sc.mul;
+    if (sc.cap) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[rt][r] = tanhf(u[r] * sc.cap_in) * sc.cap_out;
-      } else {
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[rt][r] = u[r] * sc.mul;
-      }
-      if (table) {
-        const float* w = win + 32 * rt + (NCOL - 1) - tl;
+        for (int r = 0; r < 16; ++r) s[rt][r] = cap_tanh<EXACT>(s[rt][r] * sc.cap_in) * sc.cap_out;
+      mul = 1.f;
+    }
+    if (table) {
+      const float* w = win[buf] + (NCOL - 1) - tl;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[rt][r] += w[pos_of(r, h)];
-      }
-      if (s0 < flo || s0 + N > fhi) {
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[rt][r] = fmaf(s[rt][r], mul, w[32 * rt + pos_of(r, h)]);
+      mul = 1.f;
+    }
+    if (s0 < flo || s0 + N > fhi) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int p = s0 + 32 * rt + pos_of(r, h);
-          s[rt][r] = p >= iv.x && p < iv.y ? s[rt][r] : -INFINITY;
+          const unsigned p = s0 + 32 * rt + pos_of(r, h) - iv.x;
+          s[rt][r] = p < (unsigned)(iv.y - iv.x) ? s[rt][r] : -INFINITY;
         }
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[rt][r]);
     }
-    mt = fmaxf(mt, __shfl_xor(mt, 32));
-    const float m1 = fmaxf(m, mt), ms = m1 == -INFINITY ? 0.f : m1 - PUP<E>;
-    const float alpha = __builtin_amdgcn_exp2f(m - (ms + PUP<E>));
-    m = m1;
-    l *= alpha;
+    float mt = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
+      for (int r = 0; r < 16; r += 2) mt = fmaxf(fmaxf(s[rt][r], s[rt][r + 1]), mt);
+    mt = fmaxf(mt, __shfl_xor(mt, 32)) * mul;
+    if (__any(mt > m + LAZY)) {
+      const float m1 = fmaxf(m, mt), alpha = __builtin_amdgcn_exp2f(m1 == -INFINITY ? 0.f : m - m1);
+      m = m1;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
+    }
+    const float ms = m == -INFINITY ? 0.f : m - PUP<E>;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+      float ls = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[rt][r] = __builtin_amdgcn_exp2f(s[rt][r] - ms);
-        l += s[rt][r];
+        s[rt][r] = __builtin_amdgcn_exp2f(fmaf(s[rt][r], mul, -ms));
+        ls += s[rt][r];
       }
+      l += ls;
       if (a.seed) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const unsigned long long z = draw_word(draws, (unsigned long long)((s0 + 32 * rt + pos_of(4 * w, h)) >> 2));
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (((unsigned)(z >> (16 * j)) & 0xffffu) < thr) s[rt][4 * w + j] = 0.f;
+          for (int j = 0; j < 4; ++j) s[rt][4 * w + j] = dropped(z, j, thr) ? 0.f : s[rt][4 * w + j];
         }
       }
-      if (sizeof(E) == 2 && a.out32) mul_rows<E, DP, true>(acc, vs, rt, s[rt], lane);
-      else mul_rows<E, DP>(acc, vs, rt, s[rt], lane);
+      mul_rows<E, DP, sizeof(E) == 4 || !EXACT ? 1 : __is_same(E, bf16_t) ? 3 : 2>(acc, vs, rt, s[rt], lane);
     }
   }
 
@@ -126,9 +153,9 @@ __global__ __launch_bounds__(256) void fwd_kernel(svc_attn_scored_t a, int n_til
   float inv = l > 0.f ? 1.f / l : 0.f;
   if (l != l) inv = l;                                  // nan scores give nan, as they would in any softmax
   if (a.seed) inv *= 65536.f / (65536.f - (float)thr);
-  if (a.lse && h == 0) a.lse[(long long)bh * a.Tq + t] = some ? m - PUP<E> + __builtin_amdgcn_logf(l) : 0.f;
+  if (a.lse && h == 0) a.lse[bh * a.Tq + t] = some ? m - PUP<E> + __builtin_amdgcn_logf(l) : 0.f;
   E* op = (E*)a.out + b * a.o_bs + (long long)head * a.dk * a.o_cs + t;
-  float* fp = a.out32 ? a.out32 + (long long)bh * a.dk * a.Tq + t : nullptr;
+  float* fp = a.out32 ? a.out32 + bh * a.dk * a.Tq + t : nullptr;
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -154,27 +181,30 @@ int check_args(const svc_attn_scored_t* a, bool backward) {
   SVC_REQUIRE(!a->prefix || (a->causal && a->window < 0), "attn_scored: a prefix goes with a causal mask and no window");
   SVC_REQUIRE(!a->bias || (a->bias_w >= 0 && a->bias_w < (1 << 29) && (a->bias_heads == 1 || a->bias_heads == a->H)),
               "attn_scored: bias of %d heads, width %d", a->bias_heads, a->bias_w);
-  SVC_REQUIRE(a->scale == a->scale && a->softcap >= 0.f && a->softcap < INFINITY, "attn_scored: scale %g, softcap %g", a->scale, a->softcap);
+  SVC_REQUIRE(a->scale > 0.f && a->scale < INFINITY && a->softcap >= 0.f && a->softcap < INFINITY, "attn_scored: scale %g, softcap %g", a->scale, a->softcap);
   SVC_REQUIRE(!a->seed || (a->p_drop >= 0.f && a->p_drop <= 0.99f), "attn_scored: dropout rate %g (0..0.99)", a->p_drop);
   if (a->B == 0 || a->Tq == 0) return SVC_OK;
   SVC_REQUIRE(a->q && a->k && a->v, "attn_scored: q, k, v");
   if (!backward) SVC_REQUIRE(a->out, "attn_scored: out");
   if (backward) {
-    SVC_REQUIRE(a->dout && a->lse && a->dq && a->dk_ && a->dv && (a->out || a->out32), "attn_scored_bwd: dout, lse, out or out32, dq, dk, dv");
-    SVC_REQUIRE(!a->dbias || (a->bias && (a->dtype == SVC_F32 || a->out32)), "attn_scored_bwd: dbias needs bias, and out32 for 16-bit types");
+    SVC_REQUIRE(a->dout && a->lse && a->dq && a->dk_ && a->dv && (a->dtype == SVC_F32 ? a->out != nullptr : a->out32 != nullptr),
+                "attn_scored_bwd: dout, lse, %s, dq, dk, dv", a->dtype == SVC_F32 ? "out" : "out32");
+    SVC_REQUIRE(!a->dbias || a->bias, "attn_scored_bwd: dbias without bias");
   }
   const long long need = svc_attn_scored_ws_bytes(a, backward);
   SVC_REQUIRE(need == 0 || (a->ws && a->ws_bytes >= need && ((size_t)a->ws & 15) == 0), "attn_scored: workspace of %lld bytes needed, %lld given",
               need, a->ws ? a->ws_bytes : 0LL);
   const long long groups = (long long)a->B * a->H * svc::cdiv(a->Tk, 32);
-  SVC_REQUIRE(groups < (1LL << 31), "attn_scored: %lld tiles", groups);
+  SVC_REQUIRE(groups < (1LL << 30), "attn_scored: %lld tiles", groups);
   return SVC_OK;
 }
 
 template <typename E, int DP>
 static void launch_fwd(const svc_attn_scored_t& a, hipStream_t s) {
   const int n_tiles = (a.Tq + NCOL - 1) / NCOL;
-  hipLaunchKernelGGL((fwd_kernel<E, DP>), dim3((unsigned)(a.B * a.H * n_tiles)), dim3(256), 0, s, a, n_tiles);
+  const unsigned grid = (unsigned)grid_of((long long)a.B * a.G, a.H / a.G, n_tiles);
+  if (sizeof(E) == 4 || a.exact) hipLaunchKernelGGL((fwd_kernel<E, DP, true>), dim3(grid), dim3(256), 0, s, a, n_tiles);
+  else hipLaunchKernelGGL((fwd_kernel<E, DP, sizeof(E) == 4>), dim3(grid), dim3(256), 0, s, a, n_tiles);
 }
 template <typename E>
 static void pick_fwd(const svc_attn_scored_t& a, hipStream_t s) {

@@ -120,7 +120,7 @@ class AttnScored(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "out32", "lse", "bias", "lengths", "offsets", "docs", "prefix", "seed", "dout",
                                           "dq", "dk_", "dv", "dbias", "ws")] + \
         [(n, C.c_longlong) for n in ("ws_bytes", "q_bs", "q_cs", "k_bs", "k_cs", "v_bs", "v_cs", "o_bs", "o_cs", "do_bs", "do_cs")] + \
-        [(n, C.c_int) for n in ("dtype", "B", "H", "G", "dk", "Tq", "Tk", "causal", "window", "n_docs", "offset", "bias_w", "bias_heads", "site")] + \
+        [(n, C.c_int) for n in ("dtype", "B", "H", "G", "dk", "Tq", "Tk", "causal", "window", "n_docs", "offset", "bias_w", "bias_heads", "site", "exact")] + \
         [(n, C.c_float) for n in ("scale", "softcap", "p_drop")]
 
 
@@ -2081,6 +2081,8 @@ def _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, pr
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     a.dtype, a.B, a.H, a.G, a.dk, a.Tq, a.Tk = code, B, n_heads, k.shape[1] // dk, dk, Tq, Tk
     a.scale = dk ** -0.5 if scale is None else scale
+    if not a.scale > 0.0:
+        raise SvcError(f"{what}: scale {scale}")
     a.softcap, a.causal = softcap or 0.0, 1 if causal else 0
     a.window = -1 if window is None else window
     if window is not None and window < 0:
@@ -2148,14 +2150,15 @@ def _scored_ws(a, backward, dev):
 def attention_scored_fwd(q, k, v, n_heads, *, bias=None, softcap=0.0, scale=None, causal=False, window=None, prefix=None, docs=None, lengths=None,
                          offset=None, draw=None, p_drop=0.0, want_dbias=False):
     """The forward of a training pass: attention_scored with attention dropout (`draw`: a HashDraw) -> (out, lse, out32), for
-    attention_scored_bwd.  out32, the unrounded output, is made for 16-bit tensors when the bias's gradient will be wanted, else None."""
+    attention_scored_bwd; out32, the unrounded output, is None for fp32 tensors.  `want_dbias`: the bias's gradient, fp32 whatever the tensors are, will be
+    asked for, so P and the cap keep fp32's precision."""
     a, dev = _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, draw, p_drop)
     out = torch.empty(q.shape, device=dev, dtype=q.dtype)
     lse = torch.empty((a.B, n_heads, a.Tq), device=dev, dtype=torch.float32)
     out32 = None
-    if want_dbias and q.dtype != torch.float32:
+    if q.dtype != torch.float32:
         out32 = torch.empty(q.shape, device=dev, dtype=torch.float32)
-        a.out32 = out32.data_ptr()
+        a.out32, a.exact = out32.data_ptr(), 1 if want_dbias else 0
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
     a.o_bs, a.o_cs = _bct_strides(out)
     ws = _scored_ws(a, 0, dev)
@@ -2165,22 +2168,20 @@ def attention_scored_fwd(q, k, v, n_heads, *, bias=None, softcap=0.0, scale=None
 
 def attention_scored_bwd(dout, q, k, v, out, lse, n_heads, *, bias=None, softcap=0.0, scale=None, causal=False, window=None, prefix=None, docs=None,
                          lengths=None, offset=None, draw=None, p_drop=0.0, want_dbias=False):
-    """Gradients of attention_scored_fwd -> (dq, dk, dv, dbias or None).  `out`: its output, out32 where it made one."""
+    """Gradients of attention_scored_fwd -> (dq, dk, dv, dbias or None).  `out`: its fp32 output (out32, or out for fp32 tensors)."""
     a, dev = _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, draw, p_drop)
     _typed("attention_scored_bwd", q, dout)
     if dout.shape != q.shape:
         raise SvcError(f"attention_scored_bwd: dout {tuple(dout.shape)} for q {tuple(q.shape)}")
     if dout.shape[2] > 1 and dout.stride(2) != 1:
         dout = dout.contiguous()
-    o = _side("attention_scored_bwd", "out", out, q.shape, torch.float32 if want_dbias else out.dtype, dev)
+    o = _side("attention_scored_bwd", "out", out, q.shape, torch.float32, dev)
     a.lse = _side("attention_scored_bwd", "lse", lse, (a.B, n_heads, a.Tq), torch.float32, dev)
-    if out.dtype == q.dtype:
+    if q.dtype == torch.float32:
         a.out = o
         a.o_bs, a.o_cs = _bct_strides(out)
-    elif out.dtype == torch.float32:
-        a.out32 = o
     else:
-        raise SvcError(f"attention_scored_bwd: out is {out.dtype}, the tensors {q.dtype}")
+        a.out32 = o
     a.dout = dout.data_ptr()
     a.do_bs, a.do_cs = _bct_strides(dout)
     if a.B == 0 or a.Tq == 0:

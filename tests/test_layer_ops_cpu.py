@@ -54,7 +54,7 @@ def _attn(**kw):
 BAD = [dict(dtype=3), dict(dtype=-1), dict(B=-1), dict(Tq=9), dict(Tq=-1), dict(Tk=1 << 30), dict(G=3), dict(G=0), dict(H=0), dict(dk=0), dict(dk=129),
        dict(offset=1), dict(offset=-1), dict(window=-2), dict(n_docs=2), dict(n_docs=-1), dict(prefix=4096), dict(prefix=4096, causal=1, window=3),
        dict(bias=4096, bias_heads=2), dict(bias=4096, bias_heads=4, bias_w=-1), dict(softcap=-1.0), dict(softcap=float("inf")),
-       dict(softcap=float("nan")), dict(scale=float("nan")), dict(seed=4096, p_drop=1.0), dict(seed=4096, p_drop=-0.1), dict(seed=4096, p_drop=float("nan")),
+       dict(softcap=float("nan")), dict(scale=float("nan")), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(seed=4096, p_drop=1.0), dict(seed=4096, p_drop=-0.1), dict(seed=4096, p_drop=float("nan")),
        dict(q=None), dict(k=None), dict(v=None), dict(B=1 << 30, Tk=1 << 20)]
 
 
@@ -66,7 +66,7 @@ def test_attention_refuses(bad):
         assert b"attn_scored" in S.lib().svc_last_error()
 
 
-@pytest.mark.parametrize("bad", [dict(dout=None), dict(lse=None), dict(dq=None), dict(dk_=None), dict(dv=None), dict(out32=None, out=None), dict(bias=4096, bias_heads=4, dbias=4096, out32=None),
+@pytest.mark.parametrize("bad", [dict(dout=None), dict(lse=None), dict(dq=None), dict(dk_=None), dict(dv=None), dict(out32=None), dict(dtype=0, out=None),
                                  dict(dbias=4096), dict(ws=None), dict(ws_bytes=8), dict(ws=4100)])
 def test_attention_backward_refuses(bad):
     import svc_hip as S
