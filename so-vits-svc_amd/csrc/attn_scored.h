@@ -128,45 +128,53 @@ struct Source {                         // one head's matrix as this thread sees
   int T;                                // positions that exist
   bool pad;                             // its last row lies behind dk
   __device__ __forceinline__ void set(const E* x, long long cs, int dk, int T_, int tid) {
-    const int d = tid >> 3, c = (tid & 7) * Tile<E>::V, dl = d + DP - 32;
-    row = x + (long long)d * cs + c;
-    last = x + (long long)min(dl, dk - 1) * cs + c;
+    const int d = tid >> 3, dl = d + DP - 32;
+    row = x + (long long)d * cs;
+    last = x + (long long)min(dl, dk - 1) * cs;
     step = 32 * cs;
     T = T_;
     pad = dl >= dk;
     if (DP == 32) row = last;
   }
+  // Sixteen bytes a step, from the chunk's place or, at the row's end, from the last place that has sixteen: no branch, because a branch around loads makes
+  // the compiler wait for them where its sides meet again.  (Rows of fewer than sixteen bytes are read by `commit`.)
   __device__ __forceinline__ void fetch(Pre<E, DP>& f, int p0, int tid) const {
     constexpr int S = DP / 32, V = Tile<E>::V;
-    if (p0 >= 0 && p0 + Tile<E>::N <= T) {
+    if (T < V) return;
+    const int p = min(p0 + (tid & 7) * V, T - V);
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const U128 u = *(const U128*)((i == S - 1 ? last : row + i * step) + p0);
-        f.v[i] = make_uint4(u.x, u.y, u.z, u.w);
-      }
-    } else {                            // the tile at the tensor's end: whole chunks as above, the one across the end by elements
-      const int p = p0 + (tid & 7) * V;
-#pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const E* r = (i == S - 1 ? last : row + i * step) + p0;
-        union { uint4 u; E e[V]; } x;
-        x.u = make_uint4(0, 0, 0, 0);
-        if (p >= 0 && p + V <= T) {
-          const U128 u = *(const U128*)r;
-          x.u = make_uint4(u.x, u.y, u.z, u.w);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (p + e >= 0 && p + e < T) x.e[e] = r[e];
-        }
-        f.v[i] = x.u;
-      }
+    for (int i = 0; i < S; ++i) {
+      const U128 u = *(const U128*)((i == S - 1 ? last : row + i * step) + p);
+      f.v[i] = make_uint4(u.x, u.y, u.z, u.w);
     }
   }
   __device__ __forceinline__ void commit(E* lds, Pre<E, DP>& f, int p0, int beg, int end, int tid) const {
     constexpr int S = DP / 32, V = Tile<E>::V;
+    const int p = p0 + (tid & 7) * V;
+    if (p0 + Tile<E>::N > T) {          // the chunk may have been read from further left: shift it to its place
+      if (T < V) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          union { uint4 u; E e[V]; } x;
+          x.u = make_uint4(0, 0, 0, 0);
+          const E* r = i == S - 1 ? last : row + i * step;
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (p + e < T) x.e[e] = r[p + e];
+          f.v[i] = x.u;
+        }
+      } else {
+        const int by = min(max(p - (T - V), 0), V) * (int)sizeof(E) * 8;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          union { uint4 u; unsigned __int128 q; } x;
+          x.u = f.v[i];
+          x.q = by < 128 ? x.q >> by : 0;
+          f.v[i] = x.u;
+        }
+      }
+    }
     if (p0 < beg || p0 + Tile<E>::N > end) {
-      const int p = p0 + (tid & 7) * V;
       unsigned k[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -230,14 +238,15 @@ __device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typena
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.f;
   if constexpr (sizeof(E) == 4) {
-    // four sums of a quarter of the channels each: a chain's rounding errors grow with its length and with the sums it passes through
+    // two sums of half the channels each: a chain's rounding errors grow with its length and with the sums it passes through
     const float* p = lds + h * Tile<E>::P + 32 * rt + swap23(lane & 31);
-    f32x16 part[4] = {acc, acc, acc, acc};
+    f32x16 other = acc;
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) part[j] = mfma(p[2 * (j * (DP / 8) + i) * Tile<E>::P], f.v[j * (DP / 8) + i], part[j]);
-    acc = (part[0] + part[1]) + (part[2] + part[3]);
+    for (int i = 0; i < DP / 4; ++i) {
+      acc = mfma(p[2 * i * Tile<E>::P], f.v[i], acc);
+      other = mfma(p[2 * (i + DP / 4) * Tile<E>::P], f.v[i + DP / 4], other);
+    }
+    acc = acc + other;
   } else {
     const int i16 = lane & 15, c = i16 & 3;
     const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E>::P + 32 * rt + 16 * ((lane >> 4) & 1) + 4 * (((c & 1) << 1) | (c >> 1));
@@ -293,7 +302,7 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
 
 // ---- scores in units of log 2 ------------------------------------------------------------------------------------------------------------
 struct ScoreScale {
-  float mul, cap_in, cap_out;      // no cap: u * mul; else tanh(u * cap_in) * cap_out
+  float mul, cap_in, cap_exp, cap_out;      // no cap: u * mul; else tanh(u * cap_in) * cap_out; cap_exp = 2 log2(e) cap_in
   bool cap;
 };
 __device__ __forceinline__ ScoreScale score_scale(const svc_attn_scored_t& a) {
@@ -301,19 +310,26 @@ __device__ __forceinline__ ScoreScale score_scale(const svc_attn_scored_t& a) {
   s.cap = a.softcap > 0.f;
   s.mul = a.scale * LOG2E;
   s.cap_in = s.cap ? a.scale / a.softcap : 0.f;
+  s.cap_exp = s.cap_in * (2.f * LOG2E);
   s.cap_out = a.softcap * LOG2E;
   return s;
 }
 // tanh for the cap.  EXACT (fp32, and where a fp32 gradient of the bias hangs on it): the library's.  Else 1 - 2 / (exp 2x + 1), two
 // transcendental instructions: 1e-7 absolute, so 1e-7 of the cap in a score whose P and result are rounded to 2^-8 or 2^-11.
-template <bool EXACT> __device__ __forceinline__ float cap_tanh(float x) {
-  if (EXACT) return tanhf(x);
-  return fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * LOG2E)) + 1.f), 1.f);
+template <bool EXACT> __device__ __forceinline__ float cap_tanh(float u, const ScoreScale& sc) {
+  if (EXACT) return tanhf(u * sc.cap_in);
+  return fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u * sc.cap_exp) + 1.f), 1.f);
+}
+// cap * tanh(u / cap) * log2(e)
+template <bool EXACT> __device__ __forceinline__ float capped(float u, const ScoreScale& sc) {
+  if (EXACT) return cap_tanh<true>(u, sc) * sc.cap_out;
+  return fmaf(-2.f * sc.cap_out, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u * sc.cap_exp) + 1.f), sc.cap_out);
 }
 
 // The distance bias of a tile: win[j] = table[clamp(d0 + j, -W, W) + W] * log2(e) for j in [0, n), n <= 256: the tile's distances are consecutive, so the
-// table's clamped entries become one short row in LDS and a lookup an offset from a lane's own base.  Thread j fetches and commits entry j.
-__device__ __forceinline__ float bias_entry(const float* table, int W, int d0, int j) { return table[min(max(d0 + j, -W), W) + W] * LOG2E; }
+// table's clamped entries become one short row in LDS and a lookup an offset from a lane's own base.  Thread j fetches and commits entry j
+// (times log2(e) when it commits: arithmetic on a fetched value would wait for it).
+__device__ __forceinline__ float bias_entry(const float* table, int W, int d0, int j) { return table[min(max(d0 + j, -W), W) + W]; }
 
 // ---- which (item, head, tile) a workgroup works on.  Tiles from the heaviest on (the last, under a causal mask), all heads of one tile index before the
 // next; where the key heads divide by the 8 XCDs (or there are so many that it hardly matters), a key head's workgroups share one XCD and its L2.

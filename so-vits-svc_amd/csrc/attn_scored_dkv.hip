@@ -9,7 +9,7 @@ template <int J> __device__ __forceinline__ unsigned quad(unsigned v) {      // 
 
 // 128 keys of one key head a workgroup (32 a wave), walking the query tiles of its query heads that see any of them.
 template <typename E, int DP, bool EXACT>
-__global__ __launch_bounds__(256, 2) void dkv_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
+__global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1) void dkv_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
   constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
   __shared__ __align__(16) char tiles_[4 * DP * PITCH];
   __shared__ float win[2][NCOL + N];
@@ -83,15 +83,12 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(svc_attn_scored_t a, Ws ws,
     gsrc.set((const E*)a.dout + b * a.do_bs + (long long)head * a.dk * a.do_cs, a.do_cs, a.dk, a.Tq, tid);
     qsrc.fetch(qf, t0, tid);
     gsrc.fetch(gf, t0, tid);
-    if (a.bias && tid < NCOL + N)
+    if (a.bias)
       bf = bias_entry(a.bias + (a.bias_heads > 1 ? (long long)head * (2 * a.bias_w + 1) : 0), a.bias_w, c0 - (off + t0) - (N - 1), tid);
-    if (tid < N) {
-      const int t = t0 + tid;
-      const bool in = t < a.Tq;
-      lf = in ? a.lse[bh * a.Tq + t] - PUP<E> : 0.f;
-      rf = in ? ws.rowsum[bh * a.Tq + t] : 0.f;
-      vf = in ? ws.iv[(long long)b * a.Tq + t] : make_int2(0, 0);
-    }
+    const int t = min(t0 + (tid & (N - 1)), a.Tq - 1);
+    lf = a.lse[bh * a.Tq + t];
+    rf = ws.rowsum[bh * a.Tq + t];
+    vf = ws.iv[(long long)b * a.Tq + t];
   };
   int hh = 0, t0 = 0, buf = 0;
   int4 r = make_int4(0, 0, 0, 0);
@@ -103,18 +100,19 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(svc_attn_scored_t a, Ws ws,
     E* const gs = qs + DP * Tile<E>::P;
     qsrc.commit(qs, qf, t0, tbeg, tend, tid);
     gsrc.commit(gs, gf, t0, tbeg, tend, tid);
-    if (a.bias && tid < NCOL + N) win[buf][tid] = bf;
+    if (a.bias && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
     if (tid < N) {
-      lses[buf][tid] = lf;
-      rows[buf][tid] = rf;
-      ivs[buf][tid] = vf;
+      const bool in = t0 + tid < a.Tq;
+      lses[buf][tid] = in ? lf - PUP<E> : 0.f;
+      rows[buf][tid] = in ? rf : 0.f;
+      ivs[buf][tid] = in ? vf : make_int2(0, 0);
     }
     __syncthreads();
     const int head = kvh * rep + hh, now = t0;
     const bool work = r.x < w0 + 32 && r.y > w0, whole = w0 >= r.z && w0 + 32 <= r.w && now + N <= a.Tq;
     t0 += N;
     advance(hh, t0, r);
-    if (hh < rep) fetch(hh, t0);
+    fetch(min(hh, rep - 1), t0);                             // (behind the last pair: values that are not used)
     const int cur = buf;
     buf ^= 1;
     if (!work) continue;
@@ -128,7 +126,7 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(svc_attn_scored_t a, Ws ws,
       if (sc.cap) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          th[i] = cap_tanh<EXACT>(x[i] * sc.cap_in);
+          th[i] = cap_tanh<EXACT>(x[i], sc);
           x[i] = th[i] * sc.cap_out;
         }
         mul = 1.f;

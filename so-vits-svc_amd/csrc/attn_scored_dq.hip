@@ -5,7 +5,7 @@ namespace attn {
 
 // 128 queries of one head a workgroup (32 a wave), walking the key tiles that any of them sees.
 template <typename E, int DP, bool EXACT>
-__global__ __launch_bounds__(256, 2) void dq_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
+__global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1) void dq_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
   constexpr int N = Tile<E>::N, RT = Tile<E>::RT, NB = N + 32;
   __shared__ __align__(16) char tiles_[4 * DP * PITCH];
   __shared__ float win[2][NCOL + N];
@@ -94,12 +94,12 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(svc_attn_scored_t a, Ws ws, 
     if (s0 == first) __syncthreads();
     ksrc.commit(ks, kf, s0, blo, bhi, tid);
     vsrc.commit(vs, vf, s0, blo, bhi, tid);
-    if (table && tid < NCOL + N) win[buf][tid] = bf;
+    if (table && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
     __syncthreads();
-    if (s0 + N < bhi) {
+    {                                                             // (behind the last tile: values that are not used)
       ksrc.fetch(kf, s0 + N, tid);
       vsrc.fetch(vf, s0 + N, tid);
-      if (table && tid < NCOL + N) bf = bias_entry(table, W, s0 + N + d0, tid);
+      if (table) bf = bias_entry(table, W, s0 + N + d0, tid);
     }
     if (s0 >= whi || s0 + N <= wlo) continue;
 #pragma unroll
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(svc_attn_scored_t a, Ws ws, 
       if (sc.cap) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          th[r] = cap_tanh<EXACT>(x[r] * sc.cap_in);
+          th[r] = cap_tanh<EXACT>(x[r], sc);
           x[r] = th[r] * sc.cap_out;
         }
         mul = 1.f;

@@ -71,12 +71,12 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
     if (s0 == first) __syncthreads();                             // (q's columns have been read from the tiles)
     ksrc.commit(ks, kf, s0, blo, bhi, tid);
     vsrc.commit(vs, vf, s0, blo, bhi, tid);
-    if (table && tid < NCOL + N) win[buf][tid] = bf;
+    if (table && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
     __syncthreads();
-    if (s0 + N < bhi) {
+    {                                                             // (behind the last tile: values that are not used)
       ksrc.fetch(kf, s0 + N, tid);
       vsrc.fetch(vf, s0 + N, tid);
-      if (table && tid < NCOL + N) bf = bias_entry(table, a.bias_w, s0 + N + d0, tid);
+      if (table) bf = bias_entry(table, a.bias_w, s0 + N + d0, tid);
     }
     if (s0 >= whi || s0 + N <= wlo) continue;
     float s[RT][16];
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[rt][r] = cap_tanh<EXACT>(s[rt][r] * sc.cap_in) * sc.cap_out;
+        for (int r = 0; r < 16; ++r) s[rt][r] = capped<EXACT>(s[rt][r], sc);
       mul = 1.f;
     }
     if (table) {
