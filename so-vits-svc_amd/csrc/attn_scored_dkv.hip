@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
     const int cur = buf;
     buf ^= 1;
     if (!work) continue;
-#pragma unroll
+#pragma unroll 1
     for (int rt = 0; rt < RT; ++rt) {
       const f32x16 u = mul_columns<E, DP>(qs, rt, k, lane);
       f32x16 dp = mul_columns<E, DP>(gs, rt, v, lane);

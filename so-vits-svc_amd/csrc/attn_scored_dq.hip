@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1
       if (table) bf = bias_entry(table, W, s0 + N + d0, tid);
     }
     if (s0 >= whi || s0 + N <= wlo) continue;
-#pragma unroll
+#pragma unroll 1
     for (int rt = 0; rt < RT; ++rt) {
       const f32x16 u = mul_columns<E, DP>(ks, rt, q, lane);
       f32x16 dp = mul_columns<E, DP>(vs, rt, g, lane);
