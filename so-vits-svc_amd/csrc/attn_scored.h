@@ -29,13 +29,17 @@ struct __attribute__((packed, aligned(2))) U128 { unsigned x, y, z, w; };     //
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int NCOL = 128;               // columns of a workgroup: 4 waves x 32
-constexpr int PITCH = 144;              // bytes of an LDS row: 128 of data + 16, which spreads both operand reads over all banks
 
-template <typename E> struct Tile {     // positions of a staged tile row (128 bytes)
-  static constexpr int N = 128 / (int)sizeof(E);
+// A staged tile: rows of RB bytes of positions and 16 bytes more, which spreads both operand reads over all banks.  128-byte rows (64 positions of a 16-bit
+// type, 32 of fp32); 64-byte rows for the backward at 128 channels in 16 bits, whose accumulators leave no registers for a longer tile's loads.
+template <typename E, int RB = 128, int TH = 256> struct Tile {
+  static constexpr int N = RB / (int)sizeof(E);
   static constexpr int RT = N / 32;     // 32-row accumulators a tile feeds
+  static constexpr int PITCH = RB + 16;
   static constexpr int P = PITCH / (int)sizeof(E);
   static constexpr int V = 16 / (int)sizeof(E);     // positions of a 16-byte chunk
+  static constexpr int CH = RB / 16;                // chunks (lanes) of a row
+  static constexpr int RS = TH / CH;                // rows that TH threads stage in one step
 };
 
 __device__ __forceinline__ int swap23(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
@@ -118,40 +122,39 @@ __device__ __forceinline__ f32x16 mfma(float a, float b, f32x16 c) { return __bu
 
 // ---- staging: rows 0..DP-1 of X[d][p0 .. p0+N) into LDS rows of PITCH bytes, zero outside [beg, end) and behind row dk, so what lies there (unwritten
 // cache, padding) never reaches a product.  Rows may start at any alignment of their type.  In two halves, so that a tile's loads are in flight
-// while the one before is worked on: `fetch` into registers, `commit` to LDS.  A workgroup is 256 threads: 8 lanes a row, 32 rows a step.
-template <typename E, int DP> struct Pre { uint4 v[DP / 32]; };
+// while the one before is worked on: `fetch` into registers, `commit` to LDS.  By a workgroup of TH = 256 threads, or a wave by itself.
+template <typename E, int DP, int RB = 128, int TH = 256> struct Pre { uint4 v[DP / Tile<E, RB, TH>::RS]; };
 
-template <typename E, int DP>
+template <typename E, int DP, int RB = 128, int TH = 256>
 struct Source {                         // one head's matrix as this thread sees it
   const E *row, *last;                  // its row of step 0 and of the last step (whose rows may lie behind dk: the nearest row stands for them)
   long long step;                       // elements between steps
   int T;                                // positions that exist
   bool pad;                             // its last row lies behind dk
+  static constexpr int CH = Tile<E, RB, TH>::CH, RS = Tile<E, RB, TH>::RS, S = DP / RS, V = Tile<E, RB>::V;
   __device__ __forceinline__ void set(const E* x, long long cs, int dk, int T_, int tid) {
-    const int d = tid >> 3, dl = d + DP - 32;
+    const int d = tid / CH, dl = d + DP - RS;
     row = x + (long long)d * cs;
     last = x + (long long)min(dl, dk - 1) * cs;
-    step = 32 * cs;
+    step = RS * cs;
     T = T_;
     pad = dl >= dk;
-    if (DP == 32) row = last;
+    if (DP == RS) row = last;
   }
   // Sixteen bytes a step, from the chunk's place or, at the row's end, from the last place that has sixteen: no branch, because a branch around loads makes
   // the compiler wait for them where its sides meet again.  (Rows of fewer than sixteen bytes are read by `commit`.)
-  __device__ __forceinline__ void fetch(Pre<E, DP>& f, int p0, int tid) const {
-    constexpr int S = DP / 32, V = Tile<E>::V;
+  __device__ __forceinline__ void fetch(Pre<E, DP, RB, TH>& f, int p0, int tid) const {
     if (T < V) return;
-    const int p = min(p0 + (tid & 7) * V, T - V);
+    const int p = min(p0 + (tid & (CH - 1)) * V, T - V);
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const U128 u = *(const U128*)((i == S - 1 ? last : row + i * step) + p);
       f.v[i] = make_uint4(u.x, u.y, u.z, u.w);
     }
   }
-  __device__ __forceinline__ void commit(E* lds, Pre<E, DP>& f, int p0, int beg, int end, int tid) const {
-    constexpr int S = DP / 32, V = Tile<E>::V;
-    const int p = p0 + (tid & 7) * V;
-    if (p0 + Tile<E>::N > T) {          // the chunk may have been read from further left: shift it to its place
+  __device__ __forceinline__ void commit(E* lds, Pre<E, DP, RB, TH>& f, int p0, int beg, int end, int tid) const {
+    const int p = p0 + (tid & (CH - 1)) * V;
+    if (p0 + Tile<E, RB>::N > T) {          // the chunk may have been read from further left: shift it to its place
       if (T < V) {
 #pragma unroll
         for (int i = 0; i < S; ++i) {
@@ -174,7 +177,7 @@ struct Source {                         // one head's matrix as this thread sees
         }
       }
     }
-    if (p0 < beg || p0 + Tile<E>::N > end) {
+    if (p0 < beg || p0 + Tile<E, RB>::N > end) {
       unsigned k[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -185,53 +188,54 @@ struct Source {                         // one head's matrix as this thread sees
       for (int i = 0; i < S; ++i) f.v[i] = make_uint4(f.v[i].x & k[0], f.v[i].y & k[1], f.v[i].z & k[2], f.v[i].w & k[3]);
     }
     if (pad) f.v[S - 1] = make_uint4(0, 0, 0, 0);
-    char* o = (char*)lds + (tid >> 3) * PITCH + (tid & 7) * 16;
+    constexpr int PITCH = Tile<E, RB>::PITCH;
+    char* o = (char*)lds + tid / CH * PITCH + (tid & (CH - 1)) * 16;
 #pragma unroll
-    for (int i = 0; i < S; ++i) *(uint4*)(o + i * 32 * PITCH) = f.v[i];
+    for (int i = 0; i < S; ++i) *(uint4*)(o + i * RS * PITCH) = f.v[i];
   }
 };
 
 // Columns 32 sub .. 32 sub + 31 of a staged tile as a right operand that reduces over d.
-template <typename E, int DP>
+template <typename E, int DP, int RB = 128>
 __device__ __forceinline__ void read_columns(typename Frag<E>::template Head<DP>& f, const E* lds, int sub, int lane) {
   const int h = lane >> 5;
   if constexpr (sizeof(E) == 4) {
-    const float* p = lds + h * Tile<E>::P + 32 * sub + (lane & 31);
+    const float* p = lds + h * Tile<E, RB>::P + 32 * sub + (lane & 31);
 #pragma unroll
-    for (int i = 0; i < DP / 2; ++i) f.v[i] = p[2 * i * Tile<E>::P];
+    for (int i = 0; i < DP / 2; ++i) f.v[i] = p[2 * i * Tile<E, RB>::P];
   } else {
     const int i16 = lane & 15;
-    const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E>::P + 32 * sub + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+    const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E, RB>::P + 32 * sub + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
       typedef __attribute__((address_space(3))) s16x4 lds4;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * i * Tile<E>::P));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + (16 * i + 4) * Tile<E>::P));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * i * Tile<E, RB>::P));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + (16 * i + 4) * Tile<E, RB>::P));
       f.v[i] = __builtin_bit_cast(typename Frag<E>::V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
 }
 
 // A workgroup's 128 columns of X as right operands, through the LDS of four tiles (16-bit types need two); [beg, end): columns that are used.
-template <typename E, int DP>
+template <typename E, int DP, int RB = 128>
 __device__ __forceinline__ void load_columns(typename Frag<E>::template Head<DP>& f, E* lds, const E* x, long long cs, int dk, int T, int t0, int beg, int end,
                                              int tid) {
-  constexpr int N = Tile<E>::N;
-  Source<E, DP> src;
+  constexpr int N = Tile<E, RB>::N;
+  Source<E, DP, RB> src;
   src.set(x, cs, dk, T, tid);
-  Pre<E, DP> pre[NCOL / N];
+  Pre<E, DP, RB> pre[NCOL / N];
 #pragma unroll
   for (int i = 0; i < NCOL / N; ++i) src.fetch(pre[i], t0 + i * N, tid);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < NCOL / N; ++i) src.commit(lds + i * DP * Tile<E>::P, pre[i], t0 + i * N, beg, end, tid);
+  for (int i = 0; i < NCOL / N; ++i) src.commit(lds + i * DP * Tile<E, RB>::P, pre[i], t0 + i * N, beg, end, tid);
   __syncthreads();
   const int col = (tid >> 6) * 32;
-  read_columns<E, DP>(f, lds + col / N * DP * Tile<E>::P, col % N / 32, tid & 63);
+  read_columns<E, DP, RB>(f, lds + col / N * DP * Tile<E, RB>::P, col % N / 32, tid & 63);
 }
 
 // -> [row = position, column]: sum_d X[d][position] * f[d][column]: rows = positions 32 rt .. 32 rt + 31 of the staged tile
-template <typename E, int DP>
+template <typename E, int DP, int RB = 128>
 __device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typename Frag<E>::template Head<DP>& f, int lane) {
   const int h = lane >> 5;
   f32x16 acc;
@@ -239,24 +243,25 @@ __device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typena
   for (int r = 0; r < 16; ++r) acc[r] = 0.f;
   if constexpr (sizeof(E) == 4) {
     // two sums of half the channels each: a chain's rounding errors grow with its length and with the sums it passes through
-    const float* p = lds + h * Tile<E>::P + 32 * rt + swap23(lane & 31);
+    const float* p = lds + h * Tile<E, RB>::P + 32 * rt + swap23(lane & 31);
     f32x16 other = acc;
 #pragma unroll
     for (int i = 0; i < DP / 4; ++i) {
-      acc = mfma(p[2 * i * Tile<E>::P], f.v[i], acc);
-      other = mfma(p[2 * (i + DP / 4) * Tile<E>::P], f.v[i + DP / 4], other);
+      acc = mfma(p[2 * i * Tile<E, RB>::P], f.v[i], acc);
+      other = mfma(p[2 * (i + DP / 4) * Tile<E, RB>::P], f.v[i + DP / 4], other);
     }
     acc = acc + other;
   } else {
     const int i16 = lane & 15, c = i16 & 3;
-    const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E>::P + 32 * rt + 16 * ((lane >> 4) & 1) + 4 * (((c & 1) << 1) | (c >> 1));
+    const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E, RB>::P + 32 * rt + 16 * ((lane >> 4) & 1) + 4 * (((c & 1) << 1) | (c >> 1));
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
       typedef __attribute__((address_space(3))) s16x4 lds4;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * i * Tile<E>::P));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + (16 * i + 4) * Tile<E>::P));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * i * Tile<E, RB>::P));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + (16 * i + 4) * Tile<E, RB>::P));
       const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       acc = mfma(__builtin_bit_cast(typename Frag<E>::V, v), f.v[i], acc);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
   return acc;
@@ -264,16 +269,16 @@ __device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typena
 
 // out[d, column] += sum_position X[d][position] * w[position, column], w in accumulator layout (rows 32 rt .. of the tile).  16-bit types round w
 // to the type; OPS > 1: w goes in as that many operands, its rounded value, the rounded rest, and the rest of that.
-template <typename E, int DP, int OPS = 1>
+template <typename E, int DP, int OPS = 1, int RB = 128>
 __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, int rt, const float (&w)[16], int lane) {
   const int h = lane >> 5;
-  const E* p = lds + (lane & 31) * Tile<E>::P + 32 * rt + 8 * h;
+  const E* p = lds + (lane & 31) * Tile<E, RB>::P + 32 * rt + 8 * h;
   if constexpr (sizeof(E) == 4) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
-        const f32x4 v = *(const f32x4*)(p + 32 * dt * Tile<E>::P + 16 * (q >> 1) + 4 * (q & 1));
+        const f32x4 v = *(const f32x4*)(p + 32 * dt * Tile<E, RB>::P + 16 * (q >> 1) + 4 * (q & 1));
 #pragma unroll
         for (int j = 0; j < 4; ++j) out[dt] = mfma(v[j], w[4 * q + j], out[dt]);
       }
@@ -292,10 +297,11 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
       }
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
-        const typename Frag<E>::V v = *(const typename Frag<E>::V*)(p + 32 * dt * Tile<E>::P + 16 * ks);
+        const typename Frag<E>::V v = *(const typename Frag<E>::V*)(p + 32 * dt * Tile<E, RB>::P + 16 * ks);
 #pragma unroll
         for (int o = 0; o < OPS; ++o) out[dt] = mfma(v, b[o], out[dt]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -350,6 +356,14 @@ __device__ __forceinline__ Place place_of(int id, int groups, int rep, int n_til
   }
   return p;
 }
+// ---- few queries: columns are (query head of the group, query) pairs, 32 a workgroup, and the keys are split -------------------------------------
+struct Split {
+  int cols, blocks, parts;             // columns of a key head, their workgroups of 32, parts of the keys; parts = 0: fwd_kernel's way
+};
+Split split_of(const svc_attn_scored_t& a);
+void launch_split(const svc_attn_scored_t& a, const Split& p, hipStream_t s);       // attn_scored_split.hip
+long long split_ws_bytes(const svc_attn_scored_t& a, const Split& p);
+
 static inline long long grid_of(long long groups, long long rep, long long n_tiles) {
   return (by_xcd((int)groups) ? (groups + 7) / 8 * 8 : groups) * rep * n_tiles;
 }

@@ -10,8 +10,10 @@ template <int J> __device__ __forceinline__ unsigned quad(unsigned v) {      // 
 // 128 keys of one key head a workgroup (32 a wave), walking the query tiles of its query heads that see any of them.
 template <typename E, int DP, bool EXACT>
 __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1) void dkv_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
-  constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
-  __shared__ __align__(16) char tiles_[4 * DP * PITCH];
+  constexpr int RB = 128;
+  typedef Tile<E, RB> TL;
+  constexpr int N = TL::N, RT = TL::RT;
+  __shared__ __align__(16) char tiles_[4 * DP * TL::PITCH];
   __shared__ float win[2][NCOL + N];
   __shared__ __align__(16) float lses[2][N], rows[2][N];
   __shared__ __align__(16) int2 ivs[2][N];
@@ -36,8 +38,8 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
     tend = min(tend, kend - o1);
   }
   typename Frag<E>::template Head<DP> k, v;
-  load_columns<E, DP>(k, tiles, (const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, c0, kbeg, kend, tid);
-  load_columns<E, DP>(v, tiles, (const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, c0, kbeg, kend, tid);
+  load_columns<E, DP, RB>(k, tiles, (const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, c0, kbeg, kend, tid);
+  load_columns<E, DP, RB>(v, tiles, (const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, c0, kbeg, kend, tid);
   const ScoreScale sc = score_scale(a);
   unsigned thr = 0;
   float keep = 1.f;
@@ -72,8 +74,8 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
         if (r.x < c0 + NCOL && r.y > c0) return;
       }
   };
-  Source<E, DP> qsrc, gsrc;
-  Pre<E, DP> qf, gf;
+  Source<E, DP, RB> qsrc, gsrc;
+  Pre<E, DP, RB> qf, gf;
   float bf = 0.f, lf = 0.f, rf = 0.f;
   int2 vf = make_int2(0, 0);
   auto fetch = [&](int hh, int t0) {
@@ -96,8 +98,8 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
   if (hh < rep) fetch(hh, t0);
   __syncthreads();                                           // (the keys' columns have been read from the tiles)
   while (hh < rep) {
-    E* const qs = tiles + buf * 2 * DP * Tile<E>::P;
-    E* const gs = qs + DP * Tile<E>::P;
+    E* const qs = tiles + buf * 2 * DP * TL::P;
+    E* const gs = qs + DP * TL::P;
     qsrc.commit(qs, qf, t0, tbeg, tend, tid);
     gsrc.commit(gs, gf, t0, tbeg, tend, tid);
     if (a.bias && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
@@ -118,8 +120,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
     if (!work) continue;
 #pragma unroll 1
     for (int rt = 0; rt < RT; ++rt) {
-      const f32x16 u = mul_columns<E, DP>(qs, rt, k, lane);
-      f32x16 dp = mul_columns<E, DP>(gs, rt, v, lane);
+      const f32x16 u = mul_columns<E, DP, RB>(qs, rt, k, lane);
       float x[16], th[16], p[16], mul = sc.mul;
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = u[i];
@@ -148,6 +149,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] = x[i];
+      unsigned gone = 0;                                     // dropped entries' bits
       if (a.seed) {
         // A word holds the draws of four neighbouring keys, which are four neighbouring lanes: lane j of the four works out the word of row 4w + j and
         // all of them read it from there.
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
             const unsigned f = n & 2 ? g : l;
             const bool drop = (n & 1 ? f : f << 16) < thr << 16;
             p[i] = drop ? 0.f : x[i] * keep;
-            dp[i] = drop ? 0.f : dp[i] * keep;
+            gone |= drop ? 1u << i : 0u;
           };
           one(4 * w, quad<0>(lo), quad<0>(hi));
           one(4 * w + 1, quad<1>(lo), quad<1>(hi));
@@ -168,7 +170,15 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
           one(4 * w + 3, quad<3>(lo), quad<3>(hi));
         }
       }
-      mul_rows<E, DP>(av, gs, rt, p, lane);
+      // dv's product before dP's: P as an operand takes half the registers that dP will
+      __builtin_amdgcn_sched_barrier(0);
+      mul_rows<E, DP, 1, RB>(av, gs, rt, p, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16 dp = mul_columns<E, DP, RB>(gs, rt, v, lane);
+      if (a.seed) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] = gone >> i & 1 ? 0.f : dp[i] * keep;
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float g = x[i] * (dp[i] - rows[cur][32 * rt + pos_of(i, h)]);
@@ -182,7 +192,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] *= gm;
       }
-      mul_rows<E, DP>(ak, qs, rt, x, lane);
+      mul_rows<E, DP, 1, RB>(ak, qs, rt, x, lane);
     }
   }
   if (s >= a.Tk) return;

@@ -5,9 +5,11 @@ namespace attn {
 
 // 128 queries of one head a workgroup (32 a wave), walking the key tiles that any of them sees.
 template <typename E, int DP, bool EXACT>
-__global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1) void dq_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
-  constexpr int N = Tile<E>::N, RT = Tile<E>::RT, NB = N + 32;
-  __shared__ __align__(16) char tiles_[4 * DP * PITCH];
+__global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 1) void dq_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
+  constexpr int RB = sizeof(E) == 2 && DP == 128 ? 64 : 128;
+  typedef Tile<E, RB> TL;
+  constexpr int N = TL::N, RT = TL::RT, NB = N + 32;
+  __shared__ __align__(16) char tiles_[4 * DP * TL::PITCH];
   __shared__ float win[2][NCOL + N];
   __shared__ float bin_[4][2][NB];
   __shared__ int range[2][4];
@@ -41,8 +43,8 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1
   const int cbeg = min(min(cols[0][0], cols[0][1]), min(cols[0][2], cols[0][3])), cend = max(max(cols[1][0], cols[1][1]), max(cols[1][2], cols[1][3]));
 
   typename Frag<E>::template Head<DP> q, g;
-  load_columns<E, DP>(q, tiles, (const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs, a.q_cs, a.dk, a.Tq, t0, cbeg, cend, tid);
-  load_columns<E, DP>(g, tiles, (const E*)a.dout + b * a.do_bs + (long long)head * a.dk * a.do_cs, a.do_cs, a.dk, a.Tq, t0, cbeg, cend, tid);
+  load_columns<E, DP, RB>(q, tiles, (const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs, a.q_cs, a.dk, a.Tq, t0, cbeg, cend, tid);
+  load_columns<E, DP, RB>(g, tiles, (const E*)a.dout + b * a.do_bs + (long long)head * a.dk * a.do_cs, a.do_cs, a.dk, a.Tq, t0, cbeg, cend, tid);
   const float lse = some ? a.lse[bh * a.Tq + t] : 0.f, D = some ? ws.rowsum[bh * a.Tq + t] : 0.f;
   const ScoreScale sc = score_scale(a);
   const float* table = a.bias ? a.bias + (a.bias_heads > 1 ? (long long)head * (2 * a.bias_w + 1) : 0) : nullptr;
@@ -76,10 +78,10 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1
   if (a.dbias)
     for (int j = n; j < NB; j += 32) bin[j] = 0.f;
 
-  Source<E, DP> ksrc, vsrc;
+  Source<E, DP, RB> ksrc, vsrc;
   ksrc.set((const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, tid);
   vsrc.set((const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, tid);
-  Pre<E, DP> kf, vf;
+  Pre<E, DP, RB> kf, vf;
   float bf = 0.f;
   const int first = blo / N * N;
   if (first < bhi) {
@@ -89,8 +91,8 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1
   }
   int buf = 0;
   for (int s0 = first; s0 < bhi; s0 += N, buf ^= 1) {
-    E* const ks = tiles + buf * 2 * DP * Tile<E>::P;
-    E* const vs = ks + DP * Tile<E>::P;
+    E* const ks = tiles + buf * 2 * DP * TL::P;
+    E* const vs = ks + DP * TL::P;
     if (s0 == first) __syncthreads();
     ksrc.commit(ks, kf, s0, blo, bhi, tid);
     vsrc.commit(vs, vf, s0, blo, bhi, tid);
@@ -104,8 +106,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1
     if (s0 >= whi || s0 + N <= wlo) continue;
 #pragma unroll 1
     for (int rt = 0; rt < RT; ++rt) {
-      const f32x16 u = mul_columns<E, DP>(ks, rt, q, lane);
-      f32x16 dp = mul_columns<E, DP>(vs, rt, g, lane);
+      const f32x16 u = mul_columns<E, DP, RB>(ks, rt, q, lane);
       float x[16], th[16];
       float mul = sc.mul;
 #pragma unroll
@@ -124,6 +125,10 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1
         for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], mul, w[pos_of(r, h)]);
         mul = 1.f;
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, -lse));
+      __builtin_amdgcn_sched_barrier(0);                            // one product's accumulator at a time
+      f32x16 dp = mul_columns<E, DP, RB>(vs, rt, g, lane);
       if (a.seed) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -133,7 +138,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1
         }
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], mul, -lse)) * (dp[r] - D);
+      for (int r = 0; r < 16; ++r) x[r] *= dp[r] - D;
       if (s0 < flo || s0 + N > fhi) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -162,7 +167,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 96) ? 2 : 1
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] *= gs;
       }
-      mul_rows<E, DP>(acc, ks, rt, x, lane);
+      mul_rows<E, DP, 1, RB>(acc, ks, rt, x, lane);
     }
     if (live) {
       // N complete bins leave (N = 64: one a lane; N = 32: the lower half of the lanes), 32 stay

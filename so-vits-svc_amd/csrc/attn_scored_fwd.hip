@@ -10,7 +10,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
   constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
   // a maximum that grows by less than this (a factor 2^LAZY in P) leaves the accumulators as they are: P stays far from any type's range
   constexpr float LAZY = __is_same(E, f16_t) ? 4.f : 8.f;
-  __shared__ __align__(16) char tiles_[4 * DP * PITCH];
+  __shared__ __align__(16) char tiles_[4 * DP * Tile<E>::PITCH];
   __shared__ float win[2][NCOL + N];
   __shared__ int range[2][4];
   E* const tiles = (E*)tiles_;                                    // [2 buffers][k, v][DP][P]
@@ -223,7 +223,9 @@ int svc_attn_scored_fwd(const svc_attn_scored_t* a, void* stream) {
   if (rc != SVC_OK || a->B == 0 || a->Tq == 0) return rc;
   hipStream_t s = (hipStream_t)stream;
   svc::ProfScope prof(s, "attn_scored_fwd", 4.0 * a->B * a->H * (double)a->Tq * a->Tk * a->dk, 0);
-  if (a->dtype == SVC_F32) attn::pick_fwd<float>(*a, s);
+  const attn::Split p = attn::split_of(*a);
+  if (p.parts) attn::launch_split(*a, p, s);
+  else if (a->dtype == SVC_F32) attn::pick_fwd<float>(*a, s);
   else if (a->dtype == SVC_BF16) attn::pick_fwd<attn::bf16_t>(*a, s);
   else attn::pick_fwd<attn::f16_t>(*a, s);
   return svc::check_launch("svc_attn_scored_fwd");
