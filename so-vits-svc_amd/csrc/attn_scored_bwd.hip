@@ -69,24 +69,25 @@ __global__ __launch_bounds__(256) void rows_kernel(svc_attn_scored_t a, Ws w, in
   if ((lane & 31) == 0 && t32 < (a.Tq + 31) / 32) w.tiles[(long long)b * ((a.Tq + 31) / 32) + t32] = r;
 }
 
-// ---- dbias[head or 0][j] = sum of the 32-query bins over items (and heads, for a shared table), in fixed order -----------------------
-__global__ __launch_bounds__(256) void dbias_kernel(svc_attn_scored_t a, Ws ws) {
-  __shared__ double sum[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int nb = 2 * a.bias_w + 1, j = blockIdx.x * 64 + lane, head = blockIdx.y, t32 = (a.Tq + 31) / 32;
+// ---- dbias[head or 0][j] = sum of the 32-query bins over items (and heads, for a shared table), in fixed order: 16 entries x 64 strands a workgroup ------
+__global__ __launch_bounds__(1024) void dbias_kernel(svc_attn_scored_t a, Ws ws) {
+  __shared__ double sum[64][17];
+  const int x = threadIdx.x & 15, k = threadIdx.x >> 4, nb = 2 * a.bias_w + 1, j = blockIdx.x * 16 + x, head = blockIdx.y, t32 = (a.Tq + 31) / 32;
+  const bool shared = a.bias_heads == 1;
+  const int n = (shared ? a.B * a.H : a.B) * t32;              // rows of bins; the item's (and head's) rows are neighbours
   double s = 0.0;
-  if (j < nb) {
-    if (a.bias_heads > 1) {
-      for (int b = 0; b < a.B; ++b)
-        for (int i = wave; i < t32; i += 4) s += (double)ws.bins[(((long long)b * a.H + head) * t32 + i) * nb + j];
-    } else {
-      const long long n = (long long)a.B * a.H * t32;
-      for (long long i = wave; i < n; i += 4) s += (double)ws.bins[i * nb + j];
+  if (j < nb)
+    for (int i = k; i < n; i += 64) {
+      const long long row = shared ? i : ((long long)(i / t32) * a.H + head) * t32 + i % t32;
+      s += (double)ws.bins[row * nb + j];
     }
-  }
-  sum[wave][lane] = s;
+  sum[k][x] = s;
   __syncthreads();
-  if (wave == 0 && j < nb) a.dbias[(long long)head * nb + j] = (float)((sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]));
+  for (int q = 32; q > 0; q >>= 1) {
+    if (k < q) sum[k][x] += sum[k + q][x];
+    __syncthreads();
+  }
+  if (k == 0 && j < nb) a.dbias[(long long)head * nb + j] = (float)sum[0][x];
 }
 
 }  // namespace attn
@@ -112,7 +113,7 @@ int svc_attn_scored_bwd(const svc_attn_scored_t* a, void* stream) {
   else hipLaunchKernelGGL((attn::rows_kernel<attn::f16_t>), grid, dim3(256), 0, s, *a, w, n64);
   attn::launch_dq(*a, w, s);
   attn::launch_dkv(*a, w, s);
-  if (a->dbias) hipLaunchKernelGGL(attn::dbias_kernel, dim3((2 * a->bias_w + 64) / 64, a->bias_heads), dim3(256), 0, s, *a, w);
+  if (a->dbias) hipLaunchKernelGGL(attn::dbias_kernel, dim3((2 * a->bias_w + 16) / 16, a->bias_heads), dim3(1024), 0, s, *a, w);
   return svc::check_launch("svc_attn_scored_bwd");
 }
 

@@ -3,6 +3,11 @@
 
 namespace attn {
 
+// lane l's value from lane l + 1 (0x130) or l - 1 (0x138), 0 from outside the wave
+template <int CTRL> __device__ __forceinline__ float lane_shift(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
 // 128 queries of one head a workgroup (32 a wave), walking the key tiles that any of them sees.
 template <typename E, int DP, bool EXACT>
 __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 1) void dq_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
@@ -63,10 +68,12 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
 
-  // Bias gradient.  The tile's entries of one distance lie on a diagonal: lane n of half h adds register r to bin pos(r,h) - n + 31 of its
-  // half's own row, so the lanes of one instruction never meet (a half has 32 different n) and neither do waves: LDS adds in a fixed order.
-  // As the tiles advance by N keys, a wave's first N bins are complete after each tile and leave; the last 32 stay.  Distances at or
-  // beyond +-bias_w share the table's end entries and are summed in registers.
+  // Bias gradient.  A 32 x 32 block's entries of one distance lie on a diagonal: register j of eight (neighbouring positions) and lane n belong to
+  // distance j - n.  The eight are summed along their diagonals in registers by shifting lanes one step per register, downwards for the lanes n >= j
+  // and upwards for the others (neither crosses into the other half of the wave: what would is zero); the two results, 32 and 7 distances, are added to
+  // the half's own bins in LDS, 4 additions a block instead of 16 (LDS additions of every register held the kernel: train_window_fp16 267 us).  The
+  // lanes of one addition never meet, nor do waves, so the order is fixed.  As the tiles advance by N keys, a wave's first N bins are complete after
+  // each tile and leave; the last 32 stay.  Distances at or beyond +-bias_w share the table's end entries and are summed in registers.
   const int W = a.bias_w;
   float* const bin = bin_[wave][h];
   float* bins = a.dbias ? ws.bins + (bh * ((a.Tq + 31) / 32) + (t0 >> 5) + wave) * (2 * W + 1) : nullptr;
@@ -156,7 +163,16 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
           for (int r = 0; r < 16; ++r) end_hi += x[r];
         } else {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(&bin[32 * rt + pos_of(r, h) - n + 31], x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+          for (int g8 = 0; g8 < 16; g8 += 8) {
+            float dn = n >= 7 ? x[g8 + 7] : 0.f, up = n < 1 ? x[g8 + 1] : 0.f;
+#pragma unroll
+            for (int j = 6; j >= 0; --j) dn = lane_shift<0x130>(dn) + (n >= j ? x[g8 + j] : 0.f);
+#pragma unroll
+            for (int j = 2; j < 8; ++j) up = lane_shift<0x138>(up) + (n < j ? x[g8 + j] : 0.f);
+            float* const at = &bin[32 * rt + pos_of(g8, h) - n + 31];
+            __hip_atomic_fetch_add(at, dn, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+            if (n < 7) __hip_atomic_fetch_add(at + 7, up, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+          }
         }
       }
       if (sc.cap) {

@@ -1017,31 +1017,33 @@ class _AttentionScored(Function):
 
     @staticmethod
     def forward(ctx, q, k, v, bias, n_heads, opts, sides, draw):
-        out, lse, out32 = S.attention_scored_fwd(q, k, v, n_heads, bias=bias, draw=draw, want_dbias=ctx.needs_input_grad[3], **opts, **sides)
+        args, dev = S._attn_scored_args(q, k, v, n_heads, bias, draw=draw, **opts, **sides)
+        out, lse, out32 = S._scored_forward(args, dev, q, ctx.needs_input_grad[3])
         ctx.save_for_backward(q, k, v, bias, lse, out if out32 is None else out32, *sides.values())
-        ctx.cfg = (n_heads, opts, list(sides), draw)
+        ctx.cfg = (args, dev, n_heads, opts, list(sides), draw)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, bias, lse, out, *sides = ctx.saved_tensors
-        n_heads, opts, names, draw = ctx.cfg
-        dq, dk, dv, dbias = S.attention_scored_bwd(dout, q, k, v, out, lse, n_heads, bias=bias, draw=draw, want_dbias=ctx.needs_input_grad[3],
-                                                   **opts, **dict(zip(names, sides)))
-        return dq, dk, dv, dbias, None, None, None, None
+        args, dev, n_heads, opts, names, draw = ctx.cfg
+        ptrs = (args.q, args.k, args.v, args.lse, args.out32 if args.dtype else args.out, *(getattr(args, S.SIDE_FIELDS[n]) for n in names))
+        if ptrs != tuple(t.data_ptr() for t in (q, k, v, lse, out, *sides)) or (bias is not None and args.bias != bias.data_ptr()):
+            # saved-tensor hooks brought other tensors back
+            return (*S.attention_scored_bwd(dout, q, k, v, out, lse, n_heads, bias=bias, draw=draw, want_dbias=ctx.needs_input_grad[3], **opts,
+                                            **dict(zip(names, sides))), None, None, None, None)
+        return (*S._scored_backward(args, dev, dout, q, k, v, bias if ctx.needs_input_grad[3] else None), None, None, None, None)
 
 
 def attention_scored(q, k, v, n_heads, *, bias=None, softcap=0.0, scale=None, causal=False, window=None, prefix=None, docs=None, lengths=None,
                      offset=None, draw=None, p_drop=0.0):
     """svc_hip.attention_scored for training: gradients of q, k, v and the distance bias; `draw` (a svc_hip.HashDraw, whose seed stays put until
     the backward has run) and `p_drop`: dropout of the attention probabilities."""
-    opts = dict(softcap=softcap, scale=scale, causal=causal, window=window, p_drop=float(p_drop))
-    sides = {n: t for n, t in (("prefix", prefix), ("docs", docs), ("lengths", lengths)) if t is not None}
-    if isinstance(offset, torch.Tensor):
-        sides["offset"] = offset
-    else:
-        opts["offset"] = offset
+    opts = {"softcap": softcap, "scale": scale, "causal": causal, "window": window, "p_drop": p_drop}
+    sides = {}
+    for name, t in (("prefix", prefix), ("docs", docs), ("lengths", lengths), ("offset", offset)):
+        (sides if isinstance(t, torch.Tensor) else opts)[name] = t
     return _AttentionScored.apply(q, k, v, bias, n_heads, opts, sides, draw)
 
 
@@ -1050,23 +1052,27 @@ class _DropoutAddLayerNorm(Function):
 
     @staticmethod
     def forward(ctx, x, r, gamma, beta, mask, draw, p, eps):
-        y, mean, rstd = S.dropout_add_layernorm(x, r, gamma, beta, draw=draw, p=p, mask=mask, eps=eps, stats=True)
-        ctx.save_for_backward(x, r, gamma, beta, mean, rstd, mask)
-        ctx.cfg = (draw, p, eps)
+        args, dev = S._junction_args(x, r, gamma, beta, mask, draw, p, eps)
+        x, r = _c(x), None if r is None else _c(r)
+        y, st = S._junction_forward(args, dev, x, r, True)
+        ctx.save_for_backward(x, r, gamma, beta, st, mask)
+        ctx.cfg = (args, dev, draw, p, eps)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, r, gamma, beta, mean, rstd, mask = ctx.saved_tensors
-        draw, p, eps = ctx.cfg
-        dx, dr, dgamma, dbeta = S.dropout_add_layernorm_bwd(dy, x, r, gamma, beta, mean, rstd, draw=draw, p=p, mask=mask, eps=eps)
-        return dx, dr, dgamma, dbeta, None, None, None, None
+        x, r, gamma, beta, st, mask = ctx.saved_tensors
+        args, dev, draw, p, eps = ctx.cfg
+        if args.gamma != gamma.data_ptr() or args.mean != st.data_ptr() or (mask is not None and args.mask != mask.data_ptr()):
+            args, dev = S._junction_args(x, r, gamma, beta, mask, draw, p, eps)     # saved-tensor hooks brought other tensors back
+            args.mean, args.rstd = st[0].data_ptr(), st[1].data_ptr()
+        return (*S._junction_backward(args, dev, dy, x, r), None, None, None, None)
 
 
 def dropout_add_layernorm(x, r, gamma, beta, *, draw=None, p=0.0, mask=None, eps=1e-5):
     """svc_hip.dropout_add_layernorm for training: gradients of x, r (may be None), gamma and beta."""
-    return _DropoutAddLayerNorm.apply(x, r, gamma, beta, mask, draw, float(p), float(eps))
+    return _DropoutAddLayerNorm.apply(x, r, gamma, beta, mask, draw, p, eps)
 
 
 class _Dropout(Function):

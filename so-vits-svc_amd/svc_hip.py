@@ -2062,6 +2062,9 @@ def _drop_args(what, a, draw, p, dev):
     return False
 
 
+SIDE_FIELDS = {"prefix": "prefix", "docs": "docs", "lengths": "lengths", "offset": "offsets"}      # a call's int32 side tensors and their fields
+
+
 def _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, draw, p_drop):
     what = "attention_scored"
     dev, code = _typed(what, q, k, v)
@@ -2153,14 +2156,18 @@ def attention_scored_fwd(q, k, v, n_heads, *, bias=None, softcap=0.0, scale=None
     attention_scored_bwd; out32, the unrounded output, is None for fp32 tensors.  `want_dbias`: the bias's gradient, fp32 whatever the tensors are, will be
     asked for, so P and the cap keep fp32's precision."""
     a, dev = _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, draw, p_drop)
+    return _scored_forward(a, dev, q, want_dbias)
+
+
+def _scored_forward(a, dev, q, want_dbias):
     out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    lse = torch.empty((a.B, n_heads, a.Tq), device=dev, dtype=torch.float32)
+    lse = torch.empty((a.B, a.H, a.Tq), device=dev, dtype=torch.float32)
     out32 = None
-    if q.dtype != torch.float32:
+    if a.dtype:
         out32 = torch.empty(q.shape, device=dev, dtype=torch.float32)
         a.out32, a.exact = out32.data_ptr(), 1 if want_dbias else 0
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
-    a.o_bs, a.o_cs = _bct_strides(out)
+    a.o_bs, a.o_cs = out.stride(0), out.stride(1)
     ws = _scored_ws(a, 0, dev)
     _launch_on(dev, lib().svc_attn_scored_fwd, a, "attention_scored_fwd")
     return out, lse, out32
@@ -2170,26 +2177,31 @@ def attention_scored_bwd(dout, q, k, v, out, lse, n_heads, *, bias=None, softcap
                          lengths=None, offset=None, draw=None, p_drop=0.0, want_dbias=False):
     """Gradients of attention_scored_fwd -> (dq, dk, dv, dbias or None).  `out`: its fp32 output (out32, or out for fp32 tensors)."""
     a, dev = _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, draw, p_drop)
+    o = _side("attention_scored_bwd", "out", out, q.shape, torch.float32, dev)
+    a.lse = _side("attention_scored_bwd", "lse", lse, (a.B, n_heads, a.Tq), torch.float32, dev)
+    if a.dtype:
+        a.out32 = o
+    else:
+        a.out = o
+        a.o_bs, a.o_cs = out.stride(0), out.stride(1)
+    return _scored_backward(a, dev, dout, q, k, v, bias if want_dbias else None)
+
+
+def _scored_backward(a, dev, dout, q, k, v, bias):
     _typed("attention_scored_bwd", q, dout)
     if dout.shape != q.shape:
         raise SvcError(f"attention_scored_bwd: dout {tuple(dout.shape)} for q {tuple(q.shape)}")
     if dout.shape[2] > 1 and dout.stride(2) != 1:
         dout = dout.contiguous()
-    o = _side("attention_scored_bwd", "out", out, q.shape, torch.float32, dev)
-    a.lse = _side("attention_scored_bwd", "lse", lse, (a.B, n_heads, a.Tq), torch.float32, dev)
-    if q.dtype == torch.float32:
-        a.out = o
-        a.o_bs, a.o_cs = _bct_strides(out)
-    else:
-        a.out32 = o
-    a.dout = dout.data_ptr()
-    a.do_bs, a.do_cs = _bct_strides(dout)
     if a.B == 0 or a.Tq == 0:
-        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(bias) if want_dbias else None
+        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None if bias is None else torch.zeros_like(bias)
+    a.dout = dout.data_ptr()
+    a.do_bs, a.do_cs = dout.stride(0), dout.stride(1)
     dq, dk, dv = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
     a.dq, a.dk_, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     dbias = None
-    if want_dbias:
+    a.dbias = None
+    if bias is not None:
         dbias = torch.empty(bias.shape, device=dev, dtype=torch.float32)
         a.dbias = dbias.data_ptr()
     ws = _scored_ws(a, 1, dev)
@@ -2222,37 +2234,47 @@ def _junction_args(x, r, gamma, beta, mask, draw, p, eps):
 def dropout_add_layernorm(x, r, gamma, beta, *, draw=None, p=0.0, mask=None, eps=1e-5, stats=False):
     """y = LayerNorm_C(r + dropout(x)) * gamma + beta, times mask: the residual junction of a transformer layer on [B, C, T] (fp32, bf16 or fp16; gamma,
     beta fp32 [C]; mask fp32 [B, T] or [B, 1, T]; r may be None).  `draw` / `p`: dropout with svc_dropout_rng's draws.  `stats`: also return mean and
-    rstd [B, T] for dropout_add_layernorm_bwd."""
+    rstd, as one [2, B, T] tensor, for dropout_add_layernorm_bwd."""
     a, dev = _junction_args(x, r, gamma, beta, mask, draw, p, eps)
-    x, r = x.contiguous(), None if r is None else r.contiguous()
+    return _junction_forward(a, dev, x.contiguous(), None if r is None else r.contiguous(), stats)
+
+
+def _junction_forward(a, dev, x, r, stats):
     y = torch.empty(x.shape, device=dev, dtype=x.dtype)
     a.x, a.r, a.y = x.data_ptr(), None if r is None else r.data_ptr(), y.data_ptr()
     if stats:
         st = torch.empty((2, a.B, a.T), device=dev, dtype=torch.float32)
-        a.mean, a.rstd = st[0].data_ptr(), st[1].data_ptr()
+        at = st.data_ptr()
+        a.mean, a.rstd = at, at + 4 * a.B * a.T
     _launch_on(dev, lib().svc_dropout_add_layernorm_fwd, a, "dropout_add_layernorm")
-    return (y, st[0], st[1]) if stats else y
+    return (y, st) if stats else y
 
 
 def dropout_add_layernorm_bwd(dy, x, r, gamma, beta, mean, rstd, *, draw=None, p=0.0, mask=None, eps=1e-5):
     """Gradients of dropout_add_layernorm -> (dx, dr, dgamma, dbeta); without dropout dx and dr are one tensor, without r dr is None."""
-    what = "dropout_add_layernorm_bwd"
     a, dev = _junction_args(x, r, gamma, beta, mask, draw, p, eps)
-    _typed(what, x, dy)
-    if dy.shape != x.shape:
-        raise SvcError(f"{what}: dy {tuple(dy.shape)} for x {tuple(x.shape)}")
-    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
-    if x.numel() == 0:
-        return torch.zeros_like(x), None if r is None else torch.zeros_like(x), dgamma.zero_(), dbeta.zero_()
-    x, dy, r = x.contiguous(), dy.contiguous(), None if r is None else r.contiguous()
-    a.x, a.r, a.dy = x.data_ptr(), None if r is None else r.data_ptr(), dy.data_ptr()
+    what = "dropout_add_layernorm_bwd"
     a.mean, a.rstd = _side(what, "mean", mean, (a.B, a.T), torch.float32, dev), _side(what, "rstd", rstd, (a.B, a.T), torch.float32, dev)
+    return _junction_backward(a, dev, dy, x.contiguous(), None if r is None else r.contiguous())
+
+
+def _junction_backward(a, dev, dy, x, r):
+    _typed("dropout_add_layernorm_bwd", x, dy)
+    if dy.shape != x.shape:
+        raise SvcError(f"dropout_add_layernorm_bwd: dy {tuple(dy.shape)} for x {tuple(x.shape)}")
+    dparam = torch.empty((2, a.C), device=dev, dtype=torch.float32)
+    if x.numel() == 0:
+        return torch.zeros_like(x), None if r is None else torch.zeros_like(x), *dparam.zero_().unbind(0)
+    dy = dy.contiguous()
+    a.x, a.r, a.dy = x.data_ptr(), None if r is None else r.data_ptr(), dy.data_ptr()
     dr = torch.empty(x.shape, device=dev, dtype=x.dtype) if r is not None or not a.seed else None
     dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if a.seed else dr
     a.dr, a.dx = None if dr is None else dr.data_ptr(), dx.data_ptr() if a.seed else None
-    a.dgamma, a.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
+    at = dparam.data_ptr()
+    a.dgamma, a.dbeta = at, at + 4 * a.C
     n = lib().svc_dropout_add_layernorm_ws_bytes(a.B, a.C, a.T)
     ws = torch.empty((n,), device=dev, dtype=torch.uint8)
     a.ws, a.ws_bytes = ws.data_ptr(), n
-    _launch_on(dev, lib().svc_dropout_add_layernorm_bwd, a, what)
+    _launch_on(dev, lib().svc_dropout_add_layernorm_bwd, a, "dropout_add_layernorm_bwd")
+    dgamma, dbeta = dparam.unbind(0)
     return dx, dr if r is not None else None, dgamma, dbeta

@@ -102,7 +102,7 @@ def test_masked_places_are_not_used(dev):
     draw = S.HashDraw(torch.tensor([3], device=dev), 0)
 
     def go(x, r, dy):
-        y, mu, rs = S.dropout_add_layernorm(x, r, gamma, beta, mask=m, draw=draw, p=0.2, stats=True)
+        y, (mu, rs) = S.dropout_add_layernorm(x, r, gamma, beta, mask=m, draw=draw, p=0.2, stats=True)
         return (y, *S.dropout_add_layernorm_bwd(dy, x, r, gamma, beta, mu, rs, mask=m, draw=draw, p=0.2))
 
     want = go(x, r, dy)
@@ -142,7 +142,7 @@ def test_two_runs_are_bit_equal_and_replays_too(dev):
     draw = S.HashDraw(seed, 4)
 
     def step():
-        y, mu, rs = S.dropout_add_layernorm(x, r, gamma, beta, draw=draw, p=0.1, stats=True)
+        y, (mu, rs) = S.dropout_add_layernorm(x, r, gamma, beta, draw=draw, p=0.1, stats=True)
         return (y, *S.dropout_add_layernorm_bwd(dy, x, r, gamma, beta, mu, rs, draw=draw, p=0.1))
 
     want = {s: None for s in (9, 10, 11)}
