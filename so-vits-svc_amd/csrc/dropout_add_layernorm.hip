@@ -312,7 +312,7 @@ __device__ __forceinline__ void bwd_tile(const svc_dropout_add_layernorm_t& a, i
 }
 
 template <typename E, int LPR, int NR>
-__global__ __launch_bounds__(THR, 4) void junction_bwd_kernel(svc_dropout_add_layernorm_t a, int tiles_t, long long n_tiles, float* part) {
+__global__ __launch_bounds__(THR, NR > 4 ? 2 : 4) void junction_bwd_kernel(svc_dropout_add_layernorm_t a, int tiles_t, long long n_tiles, float* part) {
   constexpr int CH = THR / LPR * NR;
   __shared__ float sh[THR / 64][LPR * V];
   __shared__ float sums[2 * CH];
