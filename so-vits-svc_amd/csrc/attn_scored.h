@@ -306,6 +306,11 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
   }
 }
 
+// What a forward is for.  0: its output alone; P is rounded to the type once.  1: a 16-bit training pass (out32): the backward's row sums of dO out
+// carry P's rounding into every dS, so P goes in as two operands (train_long_bf16: dq 2.5e-3 from the exact one instead of 2.35e-3, where rounding dq
+// and dS alone leaves 2.3e-3).  2: fp32, or a 16-bit pass whose dbias, an fp32 result, will be wanted: as many operands as 24 bits take, the library's tanh.
+template <typename E, int MODE> constexpr int P_OPS = sizeof(E) == 4 || MODE == 0 ? 1 : MODE == 1 || __is_same(E, f16_t) ? 2 : 3;
+
 // ---- scores in units of log 2 ------------------------------------------------------------------------------------------------------------
 struct ScoreScale {
   float mul, cap_in, cap_exp, cap_out;      // no cap: u * mul; else tanh(u * cap_in) * cap_out; cap_exp = 2 log2(e) cap_in

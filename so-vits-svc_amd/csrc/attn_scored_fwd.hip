@@ -5,7 +5,7 @@
 namespace attn {
 
 // A workgroup owns 128 queries of one head (32 a wave) and walks the key tiles that any of them sees.
-template <typename E, int DP, bool EXACT>
+template <typename E, int DP, int MODE>
 __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_tiles) {
   constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
   // a maximum that grows by less than this (a factor 2^LAZY in P) leaves the accumulators as they are: P stays far from any type's range
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[rt][r] = capped<EXACT>(s[rt][r], sc);
+        for (int r = 0; r < 16; ++r) s[rt][r] = capped<MODE == 2>(s[rt][r], sc);
       mul = 1.f;
     }
     if (table) {
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
           for (int j = 0; j < 4; ++j) s[rt][4 * w + j] = dropped(z, j, thr) ? 0.f : s[rt][4 * w + j];
         }
       }
-      mul_rows<E, DP, sizeof(E) == 4 || !EXACT ? 1 : __is_same(E, bf16_t) ? 3 : 2>(acc, vs, rt, s[rt], lane);
+      mul_rows<E, DP, P_OPS<E, MODE>>(acc, vs, rt, s[rt], lane);
     }
   }
 
@@ -203,8 +203,10 @@ template <typename E, int DP>
 static void launch_fwd(const svc_attn_scored_t& a, hipStream_t s) {
   const int n_tiles = (a.Tq + NCOL - 1) / NCOL;
   const unsigned grid = (unsigned)grid_of((long long)a.B * a.G, a.H / a.G, n_tiles);
-  if (sizeof(E) == 4 || a.exact) hipLaunchKernelGGL((fwd_kernel<E, DP, true>), dim3(grid), dim3(256), 0, s, a, n_tiles);
-  else hipLaunchKernelGGL((fwd_kernel<E, DP, sizeof(E) == 4>), dim3(grid), dim3(256), 0, s, a, n_tiles);
+  constexpr bool F = sizeof(E) == 4;
+  if (F || a.exact) hipLaunchKernelGGL((fwd_kernel<E, DP, 2>), dim3(grid), dim3(256), 0, s, a, n_tiles);
+  else if (a.out32) hipLaunchKernelGGL((fwd_kernel<E, DP, F ? 2 : 1>), dim3(grid), dim3(256), 0, s, a, n_tiles);
+  else hipLaunchKernelGGL((fwd_kernel<E, DP, F ? 2 : 0>), dim3(grid), dim3(256), 0, s, a, n_tiles);
 }
 template <typename E>
 static void pick_fwd(const svc_attn_scored_t& a, hipStream_t s) {

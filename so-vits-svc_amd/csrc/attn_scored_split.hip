@@ -11,8 +11,8 @@ namespace attn {
 // 16-byte loads of a tile and both its matrices take 2 DP / 16 (64-byte rows) registers x 4
 template <typename E> constexpr int SPLIT_RB = sizeof(E) == 2 ? 64 : 128;
 
-template <typename E, int DP, bool EXACT>
-__global__ __launch_bounds__(256, sizeof(E) == 4 && DP > 64 ? 1 : 2) void split_kernel(svc_attn_scored_t a, Split sp) {
+template <typename E, int DP, int MODE>
+__global__ __launch_bounds__(256, DP > (sizeof(E) == 4 ? 64 : 96) ? 1 : 2) void split_kernel(svc_attn_scored_t a, Split sp) {
   constexpr int RB = SPLIT_RB<E>;
   typedef Tile<E, RB, 64> TL;
   constexpr int N = TL::N;
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && DP > 64 ? 1 : 2) void split_
     for (int r = 0; r < 16; ++r) s[r] = u[r];
     if (sc.cap) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = capped<EXACT>(s[r], sc);
+      for (int r = 0; r < 16; ++r) s[r] = capped<MODE == 2>(s[r], sc);
       mul = 1.f;
     }
     if (table) {
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && DP > 64 ? 1 : 2) void split_
         for (int j = 0; j < 4; ++j) s[4 * w + j] = dropped(z, j, thr) ? 0.f : s[4 * w + j];
       }
     }
-    mul_rows<E, DP, sizeof(E) == 4 || !EXACT ? 1 : __is_same(E, bf16_t) ? 3 : 2, RB>(acc, vs, 0, s, lane);
+    mul_rows<E, DP, P_OPS<E, MODE>, RB>(acc, vs, 0, s, lane);
   }
   l += __shfl_xor(l, 32);
 
@@ -256,8 +256,10 @@ long long split_ws_bytes(const svc_attn_scored_t& a, const Split& p) {
 template <typename E, int DP>
 static void go(const svc_attn_scored_t& a, const Split& p, hipStream_t s) {
   const dim3 grid((unsigned)((long long)a.B * a.G * p.blocks * p.parts));
-  if (sizeof(E) == 4 || a.exact) hipLaunchKernelGGL((split_kernel<E, DP, true>), grid, dim3(256), 0, s, a, p);
-  else hipLaunchKernelGGL((split_kernel<E, DP, sizeof(E) == 4>), grid, dim3(256), 0, s, a, p);
+  constexpr bool F = sizeof(E) == 4;
+  if (F || a.exact) hipLaunchKernelGGL((split_kernel<E, DP, 2>), grid, dim3(256), 0, s, a, p);
+  else if (a.out32) hipLaunchKernelGGL((split_kernel<E, DP, F ? 2 : 1>), grid, dim3(256), 0, s, a, p);
+  else hipLaunchKernelGGL((split_kernel<E, DP, F ? 2 : 0>), grid, dim3(256), 0, s, a, p);
 }
 template <typename E>
 static void pick(const svc_attn_scored_t& a, const Split& p, hipStream_t s) {
