@@ -36,9 +36,12 @@ class MultiHeadAttention(nn.Module):
         self.proximal_bias = proximal_bias
         self.proximal_init = proximal_init
         self.attn = None
-        if block_length is not None or proximal_bias or not heads_share:
-            raise NotImplementedError("block_length / proximal_bias / per-head relative embeddings are never enabled "
-                                      "on the so-vits-svc path (modules/attentions.py:33,91)")
+        if not heads_share:
+            raise NotImplementedError("per-head relative embeddings are never enabled on the so-vits-svc path (modules/attentions.py:33,91)")
+        # proximal_bias (:219-222,305-316) and block_length (:224-229) run on the scored attention, which has no relative embeddings
+        self.scored = bool(proximal_bias) or block_length is not None
+        if self.scored and window_size is not None:
+            raise NotImplementedError("proximal_bias / block_length together with a relative-position window")
         self.k_channels = channels // n_heads
         self.conv_q = Conv1d(channels, channels, 1)
         self.conv_k = Conv1d(channels, channels, 1)
@@ -82,8 +85,26 @@ class MultiHeadAttention(nn.Module):
         vec = torch.diagonal(am[:, 0], dim1=-2, dim2=-1).contiguous().float()
         outer = vec.unsqueeze(1) * vec.unsqueeze(2)
         if bool(((am[:, 0] != 0) == (outer != 0)).all()):
+            if self.scored and bool((vec[:, 1:] > vec[:, :-1]).any()):
+                raise NotImplementedError("proximal_bias / block_length with a padding mask that is not a sequence mask (ones, then zeros)")
             return MASK_PADDING, vec
         raise NotImplementedError("attention mask is neither all-ones, causal nor an outer product of a padding mask")
+
+    def _scored_options(self, mask_mode, mask_vec, T, device):
+        """The options of svc_hip.attention_scored behind this module's: the bias -log1p(|i - j|) as a table over distances, block_length as a
+        window, the padding mask as lengths.  The padding mask must be a sequence mask (ones, then zeros: commons.sequence_mask); padded queries
+        give 0 where the reference spreads them over all keys (their rows are masked behind every attention layer)."""
+        opts = {"causal": mask_mode == MASK_CAUSAL, "window": self.block_length}
+        if mask_mode == MASK_PADDING:
+            opts["lengths"] = mask_vec.sum(1).to(torch.int32)
+        if self.proximal_bias:
+            key = (T, str(device))
+            hit = self.__dict__.get("_proximal_cache")
+            if hit is None or hit[0] != key:
+                d = torch.arange(1 - T, T, device=device, dtype=torch.float32)
+                hit = self.__dict__["_proximal_cache"] = (key, (-torch.log1p(d.abs()))[None].contiguous())
+            opts["bias"] = hit[1]
+        return opts
 
     def forward_train(self, x, mask_mode, mask_vec, draws=None):
         """Reference modules/attentions.py:198-239: separate q/k/v projections, attention as GEMMs + masked softmax, and
@@ -94,6 +115,12 @@ class MultiHeadAttention(nn.Module):
             draws = DropoutDraws(self.p_dropout, self.training)
         B, C, T = x.shape
         u = draws.u((B, self.n_heads, T, T), x.device) if draws.active else None
+        if self.scored:
+            if u is not None and not isinstance(u, S.HashDraw):
+                raise NotImplementedError("attention dropout from a tensor of draws with proximal_bias / block_length")
+            q, k, v = (conv.forward_train(x) for conv in (self.conv_q, self.conv_k, self.conv_v))
+            att = A.attention_scored(q, k, v, self.n_heads, draw=u, p_drop=draws.p, **self._scored_options(mask_mode, mask_vec, T, x.device))
+            return self.conv_o.forward_train(att)
         if QKV_FUSED_TRAIN and self.conv_q.kernel_size == 1 and not self.conv_q.is_weight_norm and self.conv_q.bias is not None:
             # the three 1 x 1 projections as ONE 3C-row convolution whose rows are ordered (head, {q, k, v}, d): x has one consumer
             # (no accumulation of three input gradients), one input-gradient and one weight-gradient launch instead of three each,
@@ -125,6 +152,10 @@ class MultiHeadAttention(nn.Module):
             mask_mode, mask_vec = self._mask_mode(attn_mask, T)
         wp, b = self._qkv_packed()
         qkv = S.conv1d(x, wp, 3 * C, 1, bias=b)
+        if self.scored:
+            att = S.attention_scored(qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], self.n_heads,
+                                     **self._scored_options(mask_mode, mask_vec, T, x.device))
+            return self.conv_o.run(att)
         win = self.window_size or 0
         att = S.attention(qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], self.n_heads,
                           emb_rel_k=self.emb_rel_k[0] if win else None, emb_rel_v=self.emb_rel_v[0] if win else None,
@@ -287,16 +318,25 @@ def _encoder_forward_train(self, x, x_mask, attn_layers, norm_a, norm_b, mask_mo
     `pre_layer(i, x)`: the conditioning gate in front of each layer of a flow FFT (:49-56)."""
     m = x_mask[:, 0].contiguous() if x_mask.dim() == 3 else x_mask
     draws = DropoutDraws(self.p_dropout, self.training, dropout_u)
+    fused = attn_layers[0].scored if len(attn_layers) else False
+
+    def junction(norm, x, y):
+        """norm(x + drop(y)): the dropout, the sum and the norm as one operator where no earlier form's results are to be kept."""
+        if not fused:
+            return norm(A.add(x, draws(y)))
+        u = draws.u(tuple(y.shape), y.device) if draws.active else None
+        if u is not None and not isinstance(u, S.HashDraw):
+            return norm(A.add(x, A.dropout(y, u, draws.p)))
+        return A.dropout_add_layernorm(y, x, norm.gamma, norm.beta, draw=u, p=draws.p, eps=norm.eps)
+
     x = A.mul_bcast(x, x_mask)
     for i in range(self.n_layers):
         if pre_layer is not None:
             x = pre_layer(i, x)
         y = attn_layers[i].forward_train(x, mask_mode, m if mask_mode == MASK_PADDING else None, draws=draws)
-        y = draws(y)
-        x = norm_a[i](A.add(x, y))
+        x = junction(norm_a[i], x, y)
         y = self.ffn_layers[i].forward_train(x, x_mask, drop=draws)
-        y = draws(y)
-        x = norm_b[i](A.add(x, y))
+        x = junction(norm_b[i], x, y)
     return A.mul_bcast(x, x_mask)
 
 
