@@ -30,6 +30,25 @@ struct __attribute__((packed, aligned(2))) U128 { unsigned x, y, z, w; };     //
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int NCOL = 128;               // columns of a workgroup: 4 waves x 32
 
+// fp32 on the bf16 matrix instruction: a value is the sum of three bf16 numbers (8 + 8 + 8 bits: all of its 24, at fp32's own range), and a product the six
+// largest of their nine products, each exact in the instruction's fp32 accumulator; what is left out is 2^-24 of the product.  Six instructions for 16
+// channels take 192 cycles where the fp32 instruction's eight take 512.  x3_t is fp32 in memory and three planes of bf16 in LDS and registers.
+struct x3_t {
+  float v;
+  __device__ __forceinline__ explicit x3_t(float f) : v(f) {}
+  x3_t() = default;
+  __device__ __forceinline__ explicit operator float() const { return v; }
+};
+template <typename E> constexpr bool X3 = __is_same(E, x3_t);
+constexpr int X3_PITCH = 80;            // bytes of a plane's row of 32 positions: 64 + 16
+__device__ __forceinline__ void split3(float x, bf16_t& a, bf16_t& b, bf16_t& c) {
+  a = (bf16_t)x;
+  const float r = x - (float)a;
+  const float s = fabsf(r) < INFINITY ? r : 0.f;      // (an infinity or nan is its first part alone)
+  b = (bf16_t)s;
+  c = (bf16_t)(s - (float)b);
+}
+
 // A staged tile: rows of RB bytes of positions and 16 bytes more, which spreads both operand reads over all banks.  128-byte rows (64 positions of a 16-bit
 // type, 32 of fp32); 64-byte rows for the backward at 128 channels in 16 bits, whose accumulators leave no registers for a longer tile's loads.
 template <typename E, int RB = 128, int TH = 256> struct Tile {
@@ -40,6 +59,11 @@ template <typename E, int RB = 128, int TH = 256> struct Tile {
   static constexpr int V = 16 / (int)sizeof(E);     // positions of a 16-byte chunk
   static constexpr int CH = RB / 16;                // chunks (lanes) of a row
   static constexpr int RS = TH / CH;                // rows that TH threads stage in one step
+};
+
+template <typename E, int DP, int RB = 128> struct Staged {
+  static constexpr int SIZE = X3<E> ? 3 * DP * X3_PITCH / 4 : DP * Tile<E, RB>::P;     // elements of E from one staged matrix to the next
+  static constexpr int BUFS = X3<E> ? 1 : 2;          // three planes leave no room for a second buffer beside a second workgroup's
 };
 
 __device__ __forceinline__ int swap23(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
@@ -116,9 +140,22 @@ template <> struct Frag<f16_t> {
 // P enters a product multiplied by 2^PUP: fp16's numbers below 2^-14 lose bits, and a P of 2^-14 is an ordinary one in a long row.  256 times the
 // largest P and the largest dropout factor (100) stay below 65504.
 template <typename E> constexpr float PUP = __is_same(E, f16_t) ? 8.f : 0.f;
+template <> struct Frag<x3_t> {
+  typedef bf16x8 V;
+  template <int DP> struct Head { bf16x8 v[3][DP / 16]; };
+};
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+// the six products: the first parts' own sum, and the five small ones', which would lose their last bits in the large one step by step
+__device__ __forceinline__ void mfma6(const bf16x8 (&a)[3], bf16x8 b0, bf16x8 b1, bf16x8 b2, f32x16& large, f32x16& small) {
+  small = mfma(a[1], b1, small);
+  large = mfma(a[0], b0, large);
+  small = mfma(a[2], b0, small);
+  small = mfma(a[0], b2, small);
+  small = mfma(a[1], b0, small);
+  small = mfma(a[0], b1, small);
+}
 
 // ---- staging: rows 0..DP-1 of X[d][p0 .. p0+N) into LDS rows of PITCH bytes, zero outside [beg, end) and behind row dk, so what lies there (unwritten
 // cache, padding) never reaches a product.  Rows may start at any alignment of their type.  In two halves, so that a tile's loads are in flight
@@ -188,6 +225,28 @@ struct Source {                         // one head's matrix as this thread sees
       for (int i = 0; i < S; ++i) f.v[i] = make_uint4(f.v[i].x & k[0], f.v[i].y & k[1], f.v[i].z & k[2], f.v[i].w & k[3]);
     }
     if (pad) f.v[S - 1] = make_uint4(0, 0, 0, 0);
+    if constexpr (X3<E>) {
+      static_assert(RB == 128, "32 positions");
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        typedef bf16_t b4 __attribute__((ext_vector_type(4)));
+        const f32x4 x = __builtin_bit_cast(f32x4, f.v[i]);
+        b4 a, b, c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bf16_t u, v, w;
+          split3(x[e], u, v, w);
+          a[e] = u;
+          b[e] = v;
+          c[e] = w;
+        }
+        char* o = (char*)lds + (tid / CH + i * RS) * X3_PITCH + (tid & (CH - 1)) * 8;
+        *(b4*)o = a;
+        *(b4*)(o + DP * X3_PITCH) = b;
+        *(b4*)(o + 2 * DP * X3_PITCH) = c;
+      }
+      return;
+    }
     constexpr int PITCH = Tile<E, RB>::PITCH;
     char* o = (char*)lds + tid / CH * PITCH + (tid & (CH - 1)) * 16;
 #pragma unroll
@@ -195,53 +254,77 @@ struct Source {                         // one head's matrix as this thread sees
   }
 };
 
+// Four rows (d) of 16 columns each, transposed: lane i of 16 gets column i's four values.
+template <typename E> __device__ __forceinline__ typename Frag<E>::V read_transposed(const void* p, int four_rows) {
+  typedef __attribute__((address_space(3))) s16x4 lds4;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)((const char*)p + four_rows));
+  return __builtin_bit_cast(typename Frag<E>::V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 // Columns 32 sub .. 32 sub + 31 of a staged tile as a right operand that reduces over d.
 template <typename E, int DP, int RB = 128>
 __device__ __forceinline__ void read_columns(typename Frag<E>::template Head<DP>& f, const E* lds, int sub, int lane) {
-  const int h = lane >> 5;
-  if constexpr (sizeof(E) == 4) {
+  const int h = lane >> 5, i16 = lane & 15;
+  if constexpr (X3<E>) {
+    const char* p = (const char*)lds + (8 * h + (i16 >> 2)) * X3_PITCH + 2 * (32 * sub + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3));
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) f.v[k][i] = read_transposed<E>(p + (k * DP + 16 * i) * X3_PITCH, 4 * X3_PITCH);
+  } else if constexpr (sizeof(E) == 4) {
     const float* p = lds + h * Tile<E, RB>::P + 32 * sub + (lane & 31);
 #pragma unroll
     for (int i = 0; i < DP / 2; ++i) f.v[i] = p[2 * i * Tile<E, RB>::P];
   } else {
-    const int i16 = lane & 15;
     const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E, RB>::P + 32 * sub + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-      typedef __attribute__((address_space(3))) s16x4 lds4;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * i * Tile<E, RB>::P));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + (16 * i + 4) * Tile<E, RB>::P));
-      f.v[i] = __builtin_bit_cast(typename Frag<E>::V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
+    for (int i = 0; i < DP / 16; ++i) f.v[i] = read_transposed<E>(p + 16 * i * Tile<E, RB>::P, 4 * Tile<E, RB>::PITCH);
   }
 }
 
-// A workgroup's 128 columns of X as right operands, through the LDS of four tiles (16-bit types need two); [beg, end): columns that are used.
+// A workgroup's 128 columns of X as right operands, through the LDS of its tiles, as many at a time as there are; [beg, end): columns that are used.
 template <typename E, int DP, int RB = 128>
 __device__ __forceinline__ void load_columns(typename Frag<E>::template Head<DP>& f, E* lds, const E* x, long long cs, int dk, int T, int t0, int beg, int end,
                                              int tid) {
-  constexpr int N = Tile<E, RB>::N;
+  constexpr int N = Tile<E, RB>::N, ALL = NCOL / N, ONCE = 2 * Staged<E, DP, RB>::BUFS < ALL ? 2 * Staged<E, DP, RB>::BUFS : ALL;
+  const int col = (tid >> 6) * 32;
   Source<E, DP, RB> src;
   src.set(x, cs, dk, T, tid);
-  Pre<E, DP, RB> pre[NCOL / N];
 #pragma unroll
-  for (int i = 0; i < NCOL / N; ++i) src.fetch(pre[i], t0 + i * N, tid);
-  __syncthreads();
+  for (int at = 0; at < ALL; at += ONCE) {
+    Pre<E, DP, RB> pre[ONCE];
 #pragma unroll
-  for (int i = 0; i < NCOL / N; ++i) src.commit(lds + i * DP * Tile<E, RB>::P, pre[i], t0 + i * N, beg, end, tid);
-  __syncthreads();
-  const int col = (tid >> 6) * 32;
-  read_columns<E, DP, RB>(f, lds + col / N * DP * Tile<E, RB>::P, col % N / 32, tid & 63);
+    for (int i = 0; i < ONCE; ++i) src.fetch(pre[i], t0 + (at + i) * N, tid);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ONCE; ++i) src.commit(lds + i * Staged<E, DP, RB>::SIZE, pre[i], t0 + (at + i) * N, beg, end, tid);
+    __syncthreads();
+    if (ONCE == ALL || (col / N >= at && col / N < at + ONCE))
+      read_columns<E, DP, RB>(f, lds + (col / N - at) * Staged<E, DP, RB>::SIZE, col % N / 32, tid & 63);
+  }
 }
 
 // -> [row = position, column]: sum_d X[d][position] * f[d][column]: rows = positions 32 rt .. 32 rt + 31 of the staged tile
 template <typename E, int DP, int RB = 128>
 __device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typename Frag<E>::template Head<DP>& f, int lane) {
-  const int h = lane >> 5;
+  const int h = lane >> 5, i16 = lane & 15, c4 = 4 * (((i16 & 1) << 1) | ((i16 >> 1) & 1));
   f32x16 acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-  if constexpr (sizeof(E) == 4) {
+  if constexpr (X3<E>) {
+    const char* p = (const char*)lds + (8 * h + (i16 >> 2)) * X3_PITCH + 2 * (32 * rt + 16 * ((lane >> 4) & 1) + c4);
+    f32x16 other = acc;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      bf16x8 x[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) x[k] = read_transposed<E>(p + (k * DP + 16 * i) * X3_PITCH, 4 * X3_PITCH);
+      mfma6(x, f.v[0][i], f.v[1][i], f.v[2][i], acc, other);
+      if (i & 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    acc = acc + other;
+  } else if constexpr (sizeof(E) == 4) {
     // two sums of half the channels each: a chain's rounding errors grow with its length and with the sums it passes through
     const float* p = lds + h * Tile<E, RB>::P + 32 * rt + swap23(lane & 31);
     f32x16 other = acc;
@@ -252,15 +335,10 @@ __device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typena
     }
     acc = acc + other;
   } else {
-    const int i16 = lane & 15, c = i16 & 3;
-    const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E, RB>::P + 32 * rt + 16 * ((lane >> 4) & 1) + 4 * (((c & 1) << 1) | (c >> 1));
+    const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E, RB>::P + 32 * rt + 16 * ((lane >> 4) & 1) + c4;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
-      typedef __attribute__((address_space(3))) s16x4 lds4;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * i * Tile<E, RB>::P));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + (16 * i + 4) * Tile<E, RB>::P));
-      const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      acc = mfma(__builtin_bit_cast(typename Frag<E>::V, v), f.v[i], acc);
+      acc = mfma(read_transposed<E>(p + 16 * i * Tile<E, RB>::P, 4 * Tile<E, RB>::PITCH), f.v[i], acc);
       if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -273,7 +351,33 @@ template <typename E, int DP, int OPS = 1, int RB = 128>
 __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, int rt, const float (&w)[16], int lane) {
   const int h = lane >> 5;
   const E* p = lds + (lane & 31) * Tile<E, RB>::P + 32 * rt + 8 * h;
-  if constexpr (sizeof(E) == 4) {
+  if constexpr (X3<E>) {
+    const char* q = (const char*)lds + (lane & 31) * X3_PITCH + 2 * (32 * rt + 8 * h);
+    bf16x8 b[2][3];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      bf16_t u, v, z;
+      split3(w[e], u, v, z);
+      b[e >> 3][0][e & 7] = u;
+      b[e >> 3][1][e & 7] = v;
+      b[e >> 3][2][e & 7] = z;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) {
+      f32x16 small;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) small[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        bf16x8 x[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) x[k] = *(const bf16x8*)(q + (k * DP + 32 * dt) * X3_PITCH + 32 * ks);
+        mfma6(x, b[ks][0], b[ks][1], b[ks][2], out[dt], small);
+      }
+      out[dt] += small;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else if constexpr (sizeof(E) == 4) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll

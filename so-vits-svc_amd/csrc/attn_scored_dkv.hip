@@ -13,7 +13,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
   constexpr int RB = 128;
   typedef Tile<E, RB> TL;
   constexpr int N = TL::N, RT = TL::RT;
-  __shared__ __align__(16) char tiles_[4 * DP * TL::PITCH];
+  __shared__ __align__(16) char tiles_[2 * Staged<E, DP, RB>::BUFS * Staged<E, DP, RB>::SIZE * sizeof(E)];
   __shared__ float win[2][NCOL + N];
   __shared__ __align__(16) float lses[2][N], rows[2][N];
   __shared__ __align__(16) int2 ivs[2][N];
@@ -98,8 +98,9 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
   if (hh < rep) fetch(hh, t0);
   __syncthreads();                                           // (the keys' columns have been read from the tiles)
   while (hh < rep) {
-    E* const qs = tiles + buf * 2 * DP * TL::P;
-    E* const gs = qs + DP * TL::P;
+    if (Staged<E, DP, RB>::BUFS == 1) __syncthreads();
+    E* const qs = tiles + buf * 2 * Staged<E, DP, RB>::SIZE;
+    E* const gs = qs + Staged<E, DP, RB>::SIZE;
     qsrc.commit(qs, qf, t0, tbeg, tend, tid);
     gsrc.commit(gs, gf, t0, tbeg, tend, tid);
     if (a.bias && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
     advance(hh, t0, r);
     fetch(min(hh, rep - 1), t0);                             // (behind the last pair: values that are not used)
     const int cur = buf;
-    buf ^= 1;
+    if (Staged<E, DP, RB>::BUFS == 2) buf ^= 1;
     if (!work) continue;
 #pragma unroll 1
     for (int rt = 0; rt < RT; ++rt) {
@@ -222,11 +223,13 @@ template <typename E>
 static void pick(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
   if (a.dk <= 32) go<E, 32>(a, w, s);
   else if (a.dk <= 64) go<E, 64>(a, w, s);
-  else if (a.dk <= 96) go<E, 96>(a, w, s);
-  else go<E, 128>(a, w, s);
+  else if (a.dk <= 96 || X3<E>) go<E, 96>(a, w, s);
+  else go<E, X3<E> ? 96 : 128>(a, w, s);
 }
 void launch_dkv(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
-  if (a.dtype == SVC_F32) pick<float>(a, w, s);
+  // (three planes of k's and v's columns at 128 channels do not fit the registers beside both accumulators)
+  if (a.dtype == SVC_F32 && a.dk > 96) go<float, 128>(a, w, s);
+  else if (a.dtype == SVC_F32) pick<x3_t>(a, w, s);
   else if (a.dtype == SVC_BF16) pick<bf16_t>(a, w, s);
   else pick<f16_t>(a, w, s);
 }

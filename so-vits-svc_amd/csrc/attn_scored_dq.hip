@@ -14,7 +14,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
   constexpr int RB = sizeof(E) == 2 && DP == 128 ? 64 : 128;
   typedef Tile<E, RB> TL;
   constexpr int N = TL::N, RT = TL::RT, NB = N + 32;
-  __shared__ __align__(16) char tiles_[4 * DP * TL::PITCH];
+  __shared__ __align__(16) char tiles_[2 * Staged<E, DP, RB>::BUFS * Staged<E, DP, RB>::SIZE * sizeof(E)];
   __shared__ float win[2][NCOL + N];
   __shared__ float bin_[4][2][NB];
   __shared__ int range[2][4];
@@ -97,10 +97,10 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
     if (table && tid < NCOL + N) bf = bias_entry(table, W, first + d0, tid);
   }
   int buf = 0;
-  for (int s0 = first; s0 < bhi; s0 += N, buf ^= 1) {
-    E* const ks = tiles + buf * 2 * DP * TL::P;
-    E* const vs = ks + DP * TL::P;
-    if (s0 == first) __syncthreads();
+  for (int s0 = first; s0 < bhi; s0 += N, buf = Staged<E, DP, RB>::BUFS == 2 ? buf ^ 1 : 0) {
+    E* const ks = tiles + buf * 2 * Staged<E, DP, RB>::SIZE;
+    E* const vs = ks + Staged<E, DP, RB>::SIZE;
+    if (s0 == first || Staged<E, DP, RB>::BUFS == 1) __syncthreads();
     ksrc.commit(ks, kf, s0, blo, bhi, tid);
     vsrc.commit(vs, vf, s0, blo, bhi, tid);
     if (table && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
@@ -252,7 +252,7 @@ static void pick(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
   else go<E, 128>(a, w, s);
 }
 void launch_dq(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
-  if (a.dtype == SVC_F32) pick<float>(a, w, s);
+  if (a.dtype == SVC_F32) pick<x3_t>(a, w, s);
   else if (a.dtype == SVC_BF16) pick<bf16_t>(a, w, s);
   else pick<f16_t>(a, w, s);
 }

@@ -10,7 +10,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
   constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
   // a maximum that grows by less than this (a factor 2^LAZY in P) leaves the accumulators as they are: P stays far from any type's range
   constexpr float LAZY = __is_same(E, f16_t) ? 4.f : 8.f;
-  __shared__ __align__(16) char tiles_[4 * DP * Tile<E>::PITCH];
+  __shared__ __align__(16) char tiles_[2 * Staged<E, DP>::BUFS * Staged<E, DP>::SIZE * sizeof(E)];
   __shared__ float win[2][NCOL + N];
   __shared__ int range[2][4];
   E* const tiles = (E*)tiles_;                                    // [2 buffers][k, v][DP][P]
@@ -65,10 +65,10 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
     if (table && tid < NCOL + N) bf = bias_entry(table, a.bias_w, first + d0, tid);
   }
   int buf = 0;
-  for (int s0 = first; s0 < bhi; s0 += N, buf ^= 1) {
-    E* const ks = tiles + buf * 2 * DP * Tile<E>::P;
-    E* const vs = ks + DP * Tile<E>::P;
-    if (s0 == first) __syncthreads();                             // (q's columns have been read from the tiles)
+  for (int s0 = first; s0 < bhi; s0 += N, buf = Staged<E, DP>::BUFS == 2 ? buf ^ 1 : 0) {
+    E* const ks = tiles + buf * 2 * Staged<E, DP>::SIZE;
+    E* const vs = ks + Staged<E, DP>::SIZE;
+    if (s0 == first || Staged<E, DP>::BUFS == 1) __syncthreads();                             // (q's columns have been read from the tiles)
     ksrc.commit(ks, kf, s0, blo, bhi, tid);
     vsrc.commit(vs, vf, s0, blo, bhi, tid);
     if (table && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
@@ -227,7 +227,7 @@ int svc_attn_scored_fwd(const svc_attn_scored_t* a, void* stream) {
   svc::ProfScope prof(s, "attn_scored_fwd", 4.0 * a->B * a->H * (double)a->Tq * a->Tk * a->dk, 0);
   const attn::Split p = attn::split_of(*a);
   if (p.parts) attn::launch_split(*a, p, s);
-  else if (a->dtype == SVC_F32) attn::pick_fwd<float>(*a, s);
+  else if (a->dtype == SVC_F32) attn::pick_fwd<attn::x3_t>(*a, s);
   else if (a->dtype == SVC_BF16) attn::pick_fwd<attn::bf16_t>(*a, s);
   else attn::pick_fwd<attn::f16_t>(*a, s);
   return svc::check_launch("svc_attn_scored_fwd");
