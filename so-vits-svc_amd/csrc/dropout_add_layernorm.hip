@@ -318,8 +318,10 @@ __global__ __launch_bounds__(THR, NR > 4 ? 2 : 4) void junction_bwd_kernel(svc_d
   __shared__ float sums[2 * CH];
   for (int i = threadIdx.x; i < 2 * CH; i += THR) sums[i] = 0.f;
   __syncthreads();
-  const long long id = tile_of(blockIdx.x, gridDim.x), lo = n_tiles * id / gridDim.x, hi = n_tiles * (id + 1) / gridDim.x;
-  for (long long tile = lo; tile < hi; ++tile) {
+  // XCD x takes the tiles from x * n / 8 on, its workgroups side by side: neighbours in time share cache lines only while they are worked on together
+  // (each workgroup with a run of its own: 534 MB fetched and 282 written for 221 and 147, 768 x 1499 x 32 in bf16)
+  const long long id = blockIdx.x, xs = gridDim.x % 8 == 0 ? 8 : 1, x = id % xs, lo = n_tiles * x / xs, hi = n_tiles * (x + 1) / xs;
+  for (long long tile = lo + id / xs; tile < hi; tile += gridDim.x / xs) {
     const int b = (int)(tile / tiles_t), t0 = (int)(tile % tiles_t) * LPR * V, t = t0 + (threadIdx.x & (LPR - 1)) * V;
     if (t0 + LPR * V <= a.T) bwd_tile<E, LPR, NR, true>(a, b, t, sh, sums);
     else bwd_tile<E, LPR, NR, false>(a, b, t, sh, sums);
@@ -456,7 +458,7 @@ static Plan plan_of(int B, int C, int T, bool backward) {
   p.tiles_t = svc::cdiv(T, p.nr ? p.lpr * V : TX);
   p.n_tiles = (long long)B * p.tiles_t;
   p.blocks = (int)p.n_tiles;
-  if (backward && p.nr && p.n_tiles > 512) p.blocks = (int)svc::cdivll(p.n_tiles, svc::cdivll(p.n_tiles, 512));
+  if (backward && p.nr && p.n_tiles > 512) p.blocks = 512;
   return p;
 }
 
