@@ -754,7 +754,8 @@ int svc_cmag_bwd_f32(const float* re, const float* im, const float* mag, const f
  *   out = sum_s Z P v,  Z = keep / (1 - theta): attention dropout when seed != NULL, theta = round(65536 p_drop) / 65536 and
  *   keep[b,h,t,s] = (field s & 3 of word((b H + h) Tq + t) ceil(Tk / 4) + (s >> 2)) >= 65536 theta), word(i) the 64-bit value whose
  *   top 24 bits are svc_dropout_rng_f32's draw i of (seed, site), its fields 16 bits from the lowest.  Nothing is stored.
- * bias: fp32 [bias_heads][2 bias_w + 1] contiguous, bias_heads = H or 1; its gradient dbias has the same shape (NULL: not wanted).
+ * bias: fp32 [bias_heads][2 bias_w + 1] contiguous, bias_heads = H or 1; its gradient dbias has the same shape (NULL: not wanted).  An entry of -65504
+ * (fp16's lowest value) or below masks its distance.
  * Accumulation, softmax statistics and gradients of the bias are fp32 for every dtype; P and dS are rounded to dtype as operands.
  *
  * svc_attn_scored_fwd writes out and, when not NULL, lse [B,H,Tq] (log2 of the sum of exp2 of the scores in log2 units; 0 for a query

@@ -77,7 +77,10 @@ def attention(q, k, v, n_heads, dout=None, bias=None, softcap=0.0, scale=None, d
         at = (torch.arange(Tk) - pos[..., None]).clamp(-W, W) + W                                       # [B, Tq, Tk]
         tab = bias.detach().cpu().double().expand(H, -1)
         a = a + tab[:, at].transpose(0, 1)
-    hide = ~see[:, None]
+    hide = (~see[:, None]).expand(B, H, Tq, Tk)
+    if bias is not None:      # fp16's lowest value and below mask a distance
+        hide = hide | (tab <= -65504)[:, at].transpose(0, 1)
+        a = torch.where(hide, torch.zeros_like(a), a)
     none = hide.all(-1, keepdim=True)
     P = torch.softmax(a.masked_fill(hide & ~none, -math.inf), -1).masked_fill(hide, 0.0)
     Z = attention_keep(int(draw.seed.item()), draw.site, B, H, Tq, Tk, p_drop) if p_drop else torch.ones(())

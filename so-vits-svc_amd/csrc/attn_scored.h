@@ -446,6 +446,10 @@ template <bool EXACT> __device__ __forceinline__ float capped(float u, const Sco
 // (times log2(e) when it commits: arithmetic on a fetched value would wait for it).
 __device__ __forceinline__ float bias_entry(const float* table, int W, int d0, int j) { return table[min(max(d0 + j, -W), W) + W]; }
 
+// An entry of fp16's lowest value or below masks its distance: against any other score its exponential is 0, and a row of nothing else, whose scores such
+// an entry would absorb, counts as one without keys.
+__device__ __forceinline__ float bias_scaled(float v) { return v <= -65504.f ? -INFINITY : v * LOG2E; }
+
 // ---- which (item, head, tile) a workgroup works on.  Tiles from the heaviest on (the last, under a causal mask), all heads of one tile index before the
 // next; where the key heads divide by the 8 XCDs (or there are so many that it hardly matters), a key head's workgroups share one XCD and its L2.
 struct Place { int group, sub, tile; };           // group = item * G + key head; sub: query head of the group

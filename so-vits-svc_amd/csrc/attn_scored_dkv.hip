@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
     E* const gs = qs + Staged<E, DP, RB>::SIZE;
     qsrc.commit(qs, qf, t0, tbeg, tend, tid);
     gsrc.commit(gs, gf, t0, tbeg, tend, tid);
-    if (a.bias && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
+    if (a.bias && tid < NCOL + N) win[buf][tid] = bias_scaled(bf);
     if (tid < N) {
       const bool in = t0 + tid < a.Tq;
       lses[buf][tid] = in ? lf - PUP<E> : 0.f;

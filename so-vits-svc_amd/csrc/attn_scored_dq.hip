@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
     if (s0 == first || Staged<E, DP, RB>::BUFS == 1) __syncthreads();
     ksrc.commit(ks, kf, s0, blo, bhi, tid);
     vsrc.commit(vs, vf, s0, blo, bhi, tid);
-    if (table && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
+    if (table && tid < NCOL + N) win[buf][tid] = bias_scaled(bf);
     __syncthreads();
     {                                                             // (behind the last tile: values that are not used)
       ksrc.fetch(kf, s0 + N, tid);

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
     if (s0 == first || Staged<E, DP>::BUFS == 1) __syncthreads();                             // (q's columns have been read from the tiles)
     ksrc.commit(ks, kf, s0, blo, bhi, tid);
     vsrc.commit(vs, vf, s0, blo, bhi, tid);
-    if (table && tid < NCOL + N) win[buf][tid] = bf * LOG2E;
+    if (table && tid < NCOL + N) win[buf][tid] = bias_scaled(bf);
     __syncthreads();
     {                                                             // (behind the last tile: values that are not used)
       ksrc.fetch(kf, s0 + N, tid);
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
   float inv = l > 0.f ? 1.f / l : 0.f;
   if (l != l) inv = l;                                  // nan scores give nan, as they would in any softmax
   if (a.seed) inv *= 65536.f / (65536.f - (float)thr);
-  if (a.lse && h == 0) a.lse[bh * a.Tq + t] = some ? m - PUP<E> + __builtin_amdgcn_logf(l) : 0.f;
+  if (a.lse && h == 0) a.lse[bh * a.Tq + t] = l > 0.f || l != l ? m - PUP<E> + __builtin_amdgcn_logf(l) : 0.f;
   E* op = (E*)a.out + b * a.o_bs + (long long)head * a.dk * a.o_cs + t;
   float* fp = a.out32 ? a.out32 + bh * a.dk * a.Tq + t : nullptr;
 #pragma unroll

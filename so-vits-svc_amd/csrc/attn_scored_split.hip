@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256, DP > (sizeof(E) == 4 ? 64 : 96) ? 1 : 2) void 
     }
     if (table) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, bias[r] * LOG2E);
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, bias_scaled(bias[r]));
       mul = 1.f;
     }
     if (s0 < flo || s0 + N > fhi) {
@@ -243,8 +243,8 @@ Split split_of(const svc_attn_scored_t& a) {
   p.parts = 0;
   if (a.Tq > 64) return p;
   const long long groups = (long long)a.B * a.G * p.blocks;
-  const int span = a.window >= 0 && a.window < a.Tk ? (int)svc::cdivll(2LL * a.window + a.Tq, 1) : a.Tk;       // keys that the columns can see
-  const long long most = svc::cdiv(span < a.Tk ? span : a.Tk, 32 * 4 * 2), want = svc::cdivll(512, groups);
+  const long long seen = a.window >= 0 && 2LL * a.window + a.Tq < a.Tk ? 2LL * a.window + a.Tq : a.Tk;       // keys that the columns can see
+  const long long most = svc::cdivll(seen, 32 * 4 * 2), want = svc::cdivll(512, groups);
   p.parts = (int)(want < most ? want : most);
   if (p.parts < 1) p.parts = 1;
   return p;

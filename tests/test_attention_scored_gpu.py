@@ -360,3 +360,74 @@ def test_zero_dim_gradients_of_expanded_output(dev):
     a = torch.autograd.grad(A.attention_scored(q, k, v, 2).sum(), (q, k, v))
     b = torch.autograd.grad(A.attention_scored(q, k, v, 2), (q, k, v), torch.ones_like(q))
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("low", [-65504.0, -1e9, float(torch.finfo(torch.float32).min), float("-inf")])
+@pytest.mark.parametrize("dt", TYPES)
+def test_lowest_values_in_the_table_mask_their_distance(dev, dt, low):
+    """A table that masks distances beyond 3, some of its heads' every distance: rows with nothing left are 0 and pass nothing, as single steps too."""
+    import svc_hip as S
+    dt = TYPES[dt]
+    q, k, v, do, bias = _inputs(dev, dt, 2, 2, 1, 64, 100, 100, 8)
+    bias[:, :5], bias[:, 12:] = low, low
+    bias[1] = low
+    out, lse, o32 = S.attention_scored_fwd(q, k, v, 2, bias=bias, want_dbias=True)
+    grads = S.attention_scored_bwd(do, q, k, v, out if o32 is None else o32, lse, 2, bias=bias, want_dbias=True)
+    ref = O.attention(q, k, v, 2, dout=do, bias=bias)
+    f = _f(ref, 64, 100, 0.0)
+    for x, n, m in zip((out, *grads), ("out", "dq", "dk", "dv", "dbias"), (1.0, 2.0, 2.0, 1.0, 2.0)):
+        _check(x, ref, n, f, dt, m, m, rounded=n != "dbias")
+    assert not out[:, 64:].any() and not grads[3][1].any()
+    one = S.attention_scored(q[:, :, 99:], k, v, 2, bias=bias)
+    _check(one, {n: x[:, :, 99:] if isinstance(x, torch.Tensor) and n.endswith("out") else x for n, x in ref.items()}, "out", f, dt)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+def test_autograd_captured_and_replayed(dev, dt):
+    """A training pass through autograd in a graph (leaves made for it alone), replayed on new data."""
+    import svc_autograd as A
+    import svc_hip as S
+    dt = TYPES[dt]
+    seed = torch.tensor([1], dtype=torch.int64, device=dev)
+    draw = S.HashDraw(seed, 2)
+
+    def step(t):
+        return torch.autograd.grad(A.attention_scored(*t[:3], 4, bias=t[4], causal=True, draw=draw, p_drop=0.1), (*t[:3], t[4]), t[3])
+
+    def leaves(s):
+        return [x.requires_grad_(i != 3) for i, x in enumerate(_inputs(dev, dt, 2, 4, 2, 64, 90, 90, 7, seed=s))]
+
+    want = {}
+    for s in (0, 1):
+        seed.fill_(s)
+        want[s] = [x.clone() for x in step(leaves(s))]
+    held = leaves(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(held)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        got = step(held)
+    for s in (1, 0, 1):
+        seed.fill_(s)
+        with torch.no_grad():
+            for h, x in zip(held, leaves(s)):
+                h.copy_(x)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[s]))
+
+
+def test_second_derivatives_are_refused_and_gradients_are_per_input(dev):
+    import svc_autograd as A
+    q, k, v, _, bias = _inputs(dev, torch.float32, 1, 2, 2, 32, 20, 20, 3)
+    q.requires_grad_()
+    g, = torch.autograd.grad(A.attention_scored(q, k, v, 2, bias=bias).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    bias.requires_grad_()
+    only, = torch.autograd.grad(A.attention_scored(q.detach(), k, v, 2, bias=bias).sum(), bias)
+    assert only.shape == bias.shape
