@@ -56,23 +56,34 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
 #pragma unroll
     for (int r = 0; r < 16; ++r) ak[i][r] = av[i][r] = 0.f;
 
-  // The walk: (query head, tile) pairs whose tile has a query that sees a key of the workgroup's.
-  const int t32 = (a.Tq + 31) / 32;
+  // The walk: (query head, tile) pairs whose tile has a query that sees a key of the workgroup's.  Which tiles do is the same for every head: lane i looks
+  // at tile base + i of 64, and the walk follows the ballot's bits (looking at one tile after the other, each a dependent load, took longer than the
+  // work where masks leave few: 9 documents in 4099 queries 143 -> 134 us).
+  const int t32 = (a.Tq + 31) / 32, nt = (a.Tq + N - 1) / N;
   const int4* const spans = ws.tiles + (long long)b * t32;
-  auto span = [&](int t0) {
-    int4 r = spans[t0 >> 5];
-    if (RT == 2 && t0 + 32 < a.Tq) {
-      const int4 r1 = spans[(t0 >> 5) + 1];
-      r = make_int4(min(r.x, r1.x), max(r.y, r1.y), max(r.z, r1.z), min(r.w, r1.w));
-    }
-    return r;
-  };
-  auto advance = [&](int& hh, int& t0, int4& r) {            // to the first pair from (hh, t0) on; hh = rep: none
-    for (; hh < rep; ++hh, t0 = 0)
-      for (; t0 < a.Tq; t0 += N) {
-        r = span(t0);
-        if (r.x < c0 + NCOL && r.y > c0) return;
+  int base = -64;
+  unsigned long long left = 0;
+  int4 mine = make_int4(0, 0, 0, 0);
+  auto advance = [&](int& hh, int& t0, int4& r) {            // to the next pair; hh = rep: none
+    while (left == 0) {
+      base += 64;
+      if (base >= nt) {
+        base = 0;
+        if (++hh >= rep) return;
       }
+      const int tile = base + lane, i = min(tile * RT, t32 - 1);
+      mine = spans[i];
+      if (RT == 2) {
+        const int4 m1 = spans[min(i + 1, t32 - 1)];
+        mine = make_int4(min(mine.x, m1.x), max(mine.y, m1.y), max(mine.z, m1.z), min(mine.w, m1.w));
+      }
+      left = __ballot(tile < nt && mine.x < c0 + NCOL && mine.y > c0);
+    }
+    const int bit = __builtin_ctzll(left);
+    left &= left - 1;
+    t0 = (base + bit) * N;
+    r = make_int4(__builtin_amdgcn_readlane(mine.x, bit), __builtin_amdgcn_readlane(mine.y, bit), __builtin_amdgcn_readlane(mine.z, bit),
+                  __builtin_amdgcn_readlane(mine.w, bit));
   };
   Source<E, DP, RB> qsrc, gsrc;
   Pre<E, DP, RB> qf, gf;
@@ -113,7 +124,6 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
     __syncthreads();
     const int head = kvh * rep + hh, now = t0;
     const bool work = r.x < w0 + 32 && r.y > w0, whole = w0 >= r.z && w0 + 32 <= r.w && now + N <= a.Tq;
-    t0 += N;
     advance(hh, t0, r);
     fetch(min(hh, rep - 1), t0);                             // (behind the last pair: values that are not used)
     const int cur = buf;
