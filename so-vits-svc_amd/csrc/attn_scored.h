@@ -283,27 +283,30 @@ __device__ __forceinline__ void read_columns(typename Frag<E>::template Head<DP>
   }
 }
 
-// A workgroup's 128 columns of X as right operands, through the LDS of its tiles, as many at a time as there are; [beg, end): columns that are used.
-template <typename E, int DP, int RB = 128>
-__device__ __forceinline__ void load_columns(typename Frag<E>::template Head<DP>& f, E* lds, const E* x, long long cs, int dk, int T, int t0, int beg, int end,
-                                             int tid) {
-  constexpr int N = Tile<E, RB>::N, ALL = NCOL / N, ONCE = 2 * Staged<E, DP, RB>::BUFS < ALL ? 2 * Staged<E, DP, RB>::BUFS : ALL;
-  const int col = (tid >> 6) * 32;
+// A workgroup's 128 columns of X as right operands, through the LDS of its tiles, as many at a time as there are.  In two halves, so that a kernel asks
+// for all its columns and its first tile before it waits for any.  [beg, end): columns that are used.
+template <typename E, int DP, int RB = 128> struct Columns {
+  static constexpr int N = Tile<E, RB>::N, ALL = NCOL / N, ONCE = 2 * Staged<E, DP, RB>::BUFS < ALL ? 2 * Staged<E, DP, RB>::BUFS : ALL;
   Source<E, DP, RB> src;
-  src.set(x, cs, dk, T, tid);
+  Pre<E, DP, RB> pre[ALL];
+  __device__ __forceinline__ void fetch(const E* x, long long cs, int dk, int T, int t0, int tid) {
+    src.set(x, cs, dk, T, tid);
 #pragma unroll
-  for (int at = 0; at < ALL; at += ONCE) {
-    Pre<E, DP, RB> pre[ONCE];
-#pragma unroll
-    for (int i = 0; i < ONCE; ++i) src.fetch(pre[i], t0 + (at + i) * N, tid);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < ONCE; ++i) src.commit(lds + i * Staged<E, DP, RB>::SIZE, pre[i], t0 + (at + i) * N, beg, end, tid);
-    __syncthreads();
-    if (ONCE == ALL || (col / N >= at && col / N < at + ONCE))
-      read_columns<E, DP, RB>(f, lds + (col / N - at) * Staged<E, DP, RB>::SIZE, col % N / 32, tid & 63);
+    for (int i = 0; i < ALL; ++i) src.fetch(pre[i], t0 + i * N, tid);
   }
-}
+  __device__ __forceinline__ void settle(typename Frag<E>::template Head<DP>& f, E* lds, int t0, int beg, int end, int tid) {
+    const int col = (tid >> 6) * 32;
+#pragma unroll
+    for (int at = 0; at < ALL; at += ONCE) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < ONCE; ++i) src.commit(lds + i * Staged<E, DP, RB>::SIZE, pre[at + i], t0 + (at + i) * N, beg, end, tid);
+      __syncthreads();
+      if (ONCE == ALL || (col / N >= at && col / N < at + ONCE))
+        read_columns<E, DP, RB>(f, lds + (col / N - at) * Staged<E, DP, RB>::SIZE, col % N / 32, tid & 63);
+    }
+  }
+};
 
 // -> [row = position, column]: sum_d X[d][position] * f[d][column]: rows = positions 32 rt .. 32 rt + 31 of the staged tile
 template <typename E, int DP, int RB = 128>
@@ -481,14 +484,17 @@ static inline long long grid_of(long long groups, long long rep, long long n_til
   return (by_xcd((int)groups) ? (groups + 7) / 8 * 8 : groups) * rep * n_tiles;
 }
 
-__device__ __forceinline__ int wave_min(int v) {
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
-  return v;
-}
+// The wave's smallest / largest, by lane exchanges inside the vector unit (an exchange through LDS takes some hundred cycles, and these stand in front of
+// everything else).
+template <int CTRL> __device__ __forceinline__ int lane_of(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
 __device__ __forceinline__ int wave_max(int v) {
-  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
-  return v;
+  v = max(v, lane_of<0x111>(v));      // row_shr 1, 2, 4, 8: lane 15 of each row of 16 has the row's
+  v = max(v, lane_of<0x112>(v));
+  v = max(v, lane_of<0x114>(v));
+  v = max(v, lane_of<0x118>(v));
+  return max(max(__builtin_amdgcn_readlane(v, 15), __builtin_amdgcn_readlane(v, 31)), max(__builtin_amdgcn_readlane(v, 47), __builtin_amdgcn_readlane(v, 63)));
 }
+__device__ __forceinline__ int wave_min(int v) { return -wave_max(-v); }      // (values are positions: never the lowest int)
 
 int check_args(const svc_attn_scored_t* a, bool backward);      // attn_scored_fwd.hip
 
@@ -501,6 +507,21 @@ struct Ws {
   float* bins;     // [B*H][ceil(Tq/32)][2 bias_w + 1]  bias gradient of 32 queries
   long long bytes;
 };
+// Queries of item b that can see a key at all, and keys that can be seen (by the lengths and the outer document boundaries).
+__device__ __forceinline__ void live_range(const svc_attn_scored_t& a, int b, int& tbeg, int& tend, int& kbeg, int& kend) {
+  const int len = item_length(a, b), o = min(max(item_offset(a, b), -a.Tq), a.Tk);
+  tbeg = max(0, -o);
+  tend = max(0, min(a.Tq, len - o));
+  kbeg = 0;
+  kend = len;
+  if (a.n_docs) {
+    const int* d = a.docs + (long long)b * (a.n_docs + 1);
+    kbeg = max(0, d[0]);
+    kend = max(0, min(len, d[a.n_docs]));
+    tbeg = max(tbeg, kbeg - o);
+    tend = min(tend, kend - o);
+  }
+}
 void launch_dq(const svc_attn_scored_t& a, const Ws& w, hipStream_t s);        // attn_scored_dq.hip
 void launch_dkv(const svc_attn_scored_t& a, const Ws& w, hipStream_t s);       // attn_scored_dkv.hip
 

@@ -25,21 +25,12 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
   // (under a causal mask the first keys are the heaviest)
   const int bg = at.group, c0 = (n_tiles - 1 - at.tile) * NCOL, b = bg / a.G, kvh = bg % a.G;
   const int w0 = c0 + wave * 32, sl = wave * 32 + n, s = c0 + sl;
-  const int off = item_offset(a, b), len = item_length(a, b);
-  const float g2 = operand_scale<E>(a, ws, b, kvh, red), pup = exp2f(PUP<E>), gm = g2 / pup;
-  // queries that can see a key at all, and keys that can be seen: what lies in the others' columns is not used
-  const int o1 = min(max(off, -a.Tq), a.Tk);
-  int tbeg = max(0, -o1), tend = max(0, min(a.Tq, len - o1)), kbeg = 0, kend = len;
-  if (a.n_docs) {
-    const int* d = a.docs + (long long)b * (a.n_docs + 1);
-    kbeg = max(0, d[0]);
-    kend = max(0, min(len, d[a.n_docs]));
-    tbeg = max(tbeg, kbeg - o1);
-    tend = min(tend, kend - o1);
-  }
-  typename Frag<E>::template Head<DP> k, v;
-  load_columns<E, DP, RB>(k, tiles, (const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, c0, kbeg, kend, tid);
-  load_columns<E, DP, RB>(v, tiles, (const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, c0, kbeg, kend, tid);
+  Columns<E, DP, RB> kc, vc;
+  kc.fetch((const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, c0, tid);
+  vc.fetch((const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, c0, tid);
+  const int off = item_offset(a, b);
+  int tbeg, tend, kbeg, kend;
+  live_range(a, b, tbeg, tend, kbeg, kend);
   const ScoreScale sc = score_scale(a);
   unsigned thr = 0;
   float keep = 1.f;
@@ -107,6 +98,10 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
   int4 r = make_int4(0, 0, 0, 0);
   advance(hh, t0, r);
   if (hh < rep) fetch(hh, t0);
+  const float g2 = operand_scale<E>(a, ws, b, kvh, red), pup = exp2f(PUP<E>), gm = g2 / pup;
+  typename Frag<E>::template Head<DP> k, v;
+  kc.settle(k, tiles, c0, kbeg, kend, tid);
+  vc.settle(v, tiles, c0, kbeg, kend, tid);
   __syncthreads();                                           // (the keys' columns have been read from the tiles)
   while (hh < rep) {
     if (Staged<E, DP, RB>::BUFS == 1) __syncthreads();

@@ -17,7 +17,6 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
   __shared__ __align__(16) char tiles_[2 * Staged<E, DP, RB>::BUFS * Staged<E, DP, RB>::SIZE * sizeof(E)];
   __shared__ float win[2][NCOL + N];
   __shared__ float bin_[4][2][NB];
-  __shared__ int range[2][4];
   __shared__ float red[4];
   E* const tiles = (E*)tiles_;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, n = lane & 31;
@@ -26,31 +25,39 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
   const int b = at.group / a.G, kvh = at.group % a.G, head = kvh * (a.H / a.G) + at.sub, t0 = at.tile * NCOL;
   const long long bh = (long long)b * a.H + head;
 
-  const int tl = wave * 32 + n, t = t0 + tl;
-  const int off = item_offset(a, b);
+  const int tl = wave * 32 + n, t = t0 + tl, off = item_offset(a, b);
+  Columns<E, DP, RB> qc, gc;
+  qc.fetch((const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs, a.q_cs, a.dk, a.Tq, t0, tid);
+  gc.fetch((const E*)a.dout + b * a.do_bs + (long long)head * a.dk * a.do_cs, a.do_cs, a.dk, a.Tq, t0, tid);
   const int2 iv = t < a.Tq ? ws.iv[(long long)b * a.Tq + t] : make_int2(0, 0);
   const bool some = iv.y > iv.x;
-  const int wlo = wave_min(some ? iv.x : a.Tk), whi = wave_max(iv.y);
-  const int flo = wave_max(t < a.Tq ? (some ? iv.x : a.Tk) : 0), fhi = wave_min(t < a.Tq ? iv.y : a.Tk);
-  const int clo = wave_min(some ? t : a.Tq), chi = wave_max(some ? t + 1 : 0);
-  __shared__ int cols[2][4];
-  if (lane == 0) {
-    range[0][wave] = wlo;
-    range[1][wave] = whi;
-    cols[0][wave] = clo;
-    cols[1][wave] = chi;
+  // the four waves' key ranges, and the range that every query of this wave sees whole
+  const int t32 = (a.Tq + 31) / 32;
+  const int4* const spans = ws.tiles + (long long)b * t32;
+  int blo = a.Tk, bhi = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int4 r = spans[min((t0 >> 5) + w, t32 - 1)];
+    blo = min(blo, r.x);
+    bhi = max(bhi, r.y);
   }
-  const float gs = operand_scale<E>(a, ws, b, kvh, red);
-  __syncthreads();
-  const int blo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3]));
-  const int bhi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
-  // what q and dO hold before the first and behind the last query that sees anything is not used
-  const int cbeg = min(min(cols[0][0], cols[0][1]), min(cols[0][2], cols[0][3])), cend = max(max(cols[1][0], cols[1][1]), max(cols[1][2], cols[1][3]));
-
-  typename Frag<E>::template Head<DP> q, g;
-  load_columns<E, DP, RB>(q, tiles, (const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs, a.q_cs, a.dk, a.Tq, t0, cbeg, cend, tid);
-  load_columns<E, DP, RB>(g, tiles, (const E*)a.dout + b * a.do_bs + (long long)head * a.dk * a.do_cs, a.do_cs, a.dk, a.Tq, t0, cbeg, cend, tid);
+  const int4 mine = (t0 >> 5) + wave < t32 ? spans[min((t0 >> 5) + wave, t32 - 1)] : make_int4(a.Tk, 0, 0, a.Tk);
+  const int wlo = __builtin_amdgcn_readfirstlane(mine.x), whi = __builtin_amdgcn_readfirstlane(mine.y);
+  const int flo = __builtin_amdgcn_readfirstlane(mine.z), fhi = __builtin_amdgcn_readfirstlane(mine.w);
+  // queries that can see a key at all: what q and dO hold for the others is not used
+  int cbeg, cend, kbeg, kend;
+  live_range(a, b, cbeg, cend, kbeg, kend);
+  Source<E, DP, RB> ksrc, vsrc;
+  ksrc.set((const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, tid);
+  vsrc.set((const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, tid);
+  Pre<E, DP, RB> kf, vf;
+  const int first = blo / N * N;
+  if (first < bhi) {
+    ksrc.fetch(kf, first, tid);
+    vsrc.fetch(vf, first, tid);
+  }
   const float lse = some ? a.lse[bh * a.Tq + t] : 0.f, D = some ? ws.rowsum[bh * a.Tq + t] : 0.f;
+  const float gs = operand_scale<E>(a, ws, b, kvh, red);
   const ScoreScale sc = score_scale(a);
   const float* table = a.bias ? a.bias + (a.bias_heads > 1 ? (long long)head * (2 * a.bias_w + 1) : 0) : nullptr;
   const int d0 = -(off + t0) - (NCOL - 1);
@@ -85,17 +92,11 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
   if (a.dbias)
     for (int j = n; j < NB; j += 32) bin[j] = 0.f;
 
-  Source<E, DP, RB> ksrc, vsrc;
-  ksrc.set((const E*)a.k + b * a.k_bs + (long long)kvh * a.dk * a.k_cs, a.k_cs, a.dk, a.Tk, tid);
-  vsrc.set((const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs, a.v_cs, a.dk, a.Tk, tid);
-  Pre<E, DP, RB> kf, vf;
   float bf = 0.f;
-  const int first = blo / N * N;
-  if (first < bhi) {
-    ksrc.fetch(kf, first, tid);
-    vsrc.fetch(vf, first, tid);
-    if (table && tid < NCOL + N) bf = bias_entry(table, W, first + d0, tid);
-  }
+  if (first < bhi && table && tid < NCOL + N) bf = bias_entry(table, W, first + d0, tid);
+  typename Frag<E>::template Head<DP> q, g;
+  qc.settle(q, tiles, t0, cbeg, cend, tid);
+  gc.settle(g, tiles, t0, cbeg, cend, tid);
   int buf = 0;
   for (int s0 = first; s0 < bhi; s0 += N, buf = Staged<E, DP, RB>::BUFS == 2 ? buf ^ 1 : 0) {
     E* const ks = tiles + buf * 2 * Staged<E, DP, RB>::SIZE;
@@ -248,11 +249,13 @@ template <typename E>
 static void pick(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
   if (a.dk <= 32) go<E, 32>(a, w, s);
   else if (a.dk <= 64) go<E, 64>(a, w, s);
-  else if (a.dk <= 96) go<E, 96>(a, w, s);
-  else go<E, 128>(a, w, s);
+  else if (a.dk <= 96 || X3<E>) go<E, 96>(a, w, s);
+  else go<E, X3<E> ? 96 : 128>(a, w, s);
 }
 void launch_dq(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
-  if (a.dtype == SVC_F32) pick<x3_t>(a, w, s);
+  // (three planes of q's and dO's columns at 128 channels do not fit the registers beside the accumulators)
+  if (a.dtype == SVC_F32 && a.dk > 96) go<float, 128>(a, w, s);
+  else if (a.dtype == SVC_F32) pick<x3_t>(a, w, s);
   else if (a.dtype == SVC_BF16) pick<bf16_t>(a, w, s);
   else pick<f16_t>(a, w, s);
 }

@@ -6,7 +6,7 @@ namespace attn {
 
 // A workgroup owns 128 queries of one head (32 a wave) and walks the key tiles that any of them sees.
 template <typename E, int DP, int MODE>
-__global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_tiles) {
+__global__ __launch_bounds__(256, X3<E> && DP > 96 ? 1 : 2) void fwd_kernel(svc_attn_scored_t a, int n_tiles) {
   constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
   // a maximum that grows by less than this (a factor 2^LAZY in P) leaves the accumulators as they are: P stays far from any type's range
   constexpr float LAZY = __is_same(E, f16_t) ? 4.f : 8.f;
@@ -20,6 +20,8 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
   const int b = at.group / a.G, kvh = at.group % a.G, head = kvh * (a.H / a.G) + at.sub, t0 = at.tile * NCOL;
   const long long bh = (long long)b * a.H + head;
 
+  Columns<E, DP> qc;
+  qc.fetch((const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs, a.q_cs, a.dk, a.Tq, t0, tid);
   const int tl = wave * 32 + n, t = t0 + tl;
   const int len = item_length(a, b), off = item_offset(a, b);
   int2 iv = make_int2(0, 0);
@@ -32,8 +34,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
     range[0][wave] = wlo;
     range[1][wave] = whi;
   }
-  typename Frag<E>::template Head<DP> q;
-  load_columns<E, DP>(q, tiles, (const E*)a.q + b * a.q_bs + (long long)head * a.dk * a.q_cs, a.q_cs, a.dk, a.Tq, t0, 0, a.Tq, tid);
+  __syncthreads();
   const int blo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3]));
   const int bhi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
 
@@ -64,6 +65,8 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(svc_attn_scored_t a, int n_
     vsrc.fetch(vf, first, tid);
     if (table && tid < NCOL + N) bf = bias_entry(table, a.bias_w, first + d0, tid);
   }
+  typename Frag<E>::template Head<DP> q;
+  qc.settle(q, tiles, t0, 0, a.Tq, tid);
   int buf = 0;
   for (int s0 = first; s0 < bhi; s0 += N, buf = Staged<E, DP>::BUFS == 2 ? buf ^ 1 : 0) {
     E* const ks = tiles + buf * 2 * Staged<E, DP>::SIZE;
