@@ -108,12 +108,16 @@ __device__ __forceinline__ int2 visible(const svc_attn_scored_t& a, int b, int l
 // ---- dropout draws: the finaliser of splitmix64 over a counter, as svc_dropout_rng_f32's, with the 64 bits of a word used as four
 // 16-bit draws of four neighbouring keys: a word costs two 64-bit multiplications, more than the rest of a score's arithmetic, and
 // a 16-bit threshold holds a drop rate to 2^-17 (the kept values are scaled by the rate it stands for, so that the mean is exact).
-__device__ __forceinline__ unsigned long long draw_word(unsigned long long start, unsigned long long idx) {
-  unsigned long long z = start + idx * 0xD1B54A32D192ED03ull;
+constexpr unsigned long long DRAW_STEP = 0xD1B54A32D192ED03ull;      // from one counter to the next
+__device__ __forceinline__ unsigned long long draw_word(unsigned long long z) {      // z = start + counter * DRAW_STEP
   z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
   z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
   return z ^ (z >> 31);
 }
+// The counters of a 32 x 32 block are a lane's first one (its row, and 2 h for its half's eight keys) plus what is the same for all lanes: 64-bit
+// multiplications, quarter rate three times over, are left to the scalar unit.
+__device__ __forceinline__ unsigned long long draw_block(int s) { return (unsigned long long)(s >> 2) * DRAW_STEP; }
+__device__ __forceinline__ constexpr unsigned long long draw_group(int w) { return (unsigned long long)(4 * (w >> 1) + (w & 1)) * DRAW_STEP; }
 // draw j of a word falls under the threshold (the odd fields compare in place, the even ones shifted up)
 __device__ __forceinline__ bool dropped(unsigned long long z, int j, unsigned thr) {
   const unsigned w = (unsigned)(z >> (32 * (j >> 1)));

@@ -8,9 +8,14 @@ template <int J> __device__ __forceinline__ unsigned quad(unsigned v) {      // 
 }
 
 // 128 keys of one key head a workgroup (32 a wave), walking the query tiles of its query heads that see any of them.
-template <typename E, int DP, bool EXACT>
+template <typename E, int DP, bool EXACT, bool DROP>
 __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1) void dkv_kernel(svc_attn_scored_t a, Ws ws, int n_tiles) {
   constexpr int RB = 128;
+  // One wave a SIMD (128 channels' accumulators): dP's product is put before the exponentials, which then need not wait behind it, and the compiler orders
+  // the rest as it likes (128 channels, 4096 x 4096 causal: 1320 -> 1040 us).  Two waves fill each other's gaps and have no registers for it.
+  constexpr bool EARLY = sizeof(E) == 2 && DP > 64;
+  // (DROP is a.seed != null.  Kernels of two waves still ask for it at run time: without the branch the compiler moves the draws' registers across the
+  // products, 34 spills, 134 -> 172 us at 64 channels.  Without the draws' code at all the same kernel takes 97 us instead of 102.)
   typedef Tile<E, RB> TL;
   constexpr int N = TL::N, RT = TL::RT;
   __shared__ __align__(16) char tiles_[2 * Staged<E, DP, RB>::BUFS * Staged<E, DP, RB>::SIZE * sizeof(E)];
@@ -36,8 +41,8 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
   float keep = 1.f;
   unsigned long long start = 0;
   const unsigned long long ng = (unsigned long long)((a.Tk + 3) >> 2);
-  if (a.seed) {
-    start = draw_start(a) + (unsigned)(s >> 2) * 0xD1B54A32D192ED03ull;
+  if (DROP && (EARLY || a.seed)) {
+    start = draw_start(a) + ((unsigned long long)(s >> 2) + (unsigned long long)(8 * h + (n & 3)) * ng) * DRAW_STEP;      // row 8 h + (n & 3) of a block
     thr = (unsigned)rintf(a.p_drop * 65536.f);
     keep = 65536.f / (65536.f - (float)thr);
   }
@@ -127,6 +132,8 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
 #pragma unroll 1
     for (int rt = 0; rt < RT; ++rt) {
       const f32x16 u = mul_columns<E, DP, RB>(qs, rt, k, lane);
+      f32x16 dp;
+      if constexpr (EARLY) dp = mul_columns<E, DP, RB>(gs, rt, v, lane);
       float x[16], th[16], p[16], mul = sc.mul;
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = u[i];
@@ -156,19 +163,19 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] = x[i];
       unsigned gone = 0;                                     // dropped entries' bits
-      if (a.seed) {
+      if (DROP && (EARLY || a.seed)) {
         // A word holds the draws of four neighbouring keys, which are four neighbouring lanes: lane j of the four works out the word of row 4w + j and
-        // all of them read it from there.
-        const unsigned long long row = (unsigned long long)(((long long)b * a.H + head) * a.Tq + now + 32 * rt);
+        // all of them read it from there, each its own field (into the upper half, to compare in place).
+        const unsigned long long row = (unsigned long long)(((long long)b * a.H + head) * a.Tq + now + 32 * rt) * ng * DRAW_STEP;
+        const unsigned field = 0x01000c0cu + (n & 3) * 0x02020000u;      // bytes 2 f + 1, 2 f, zero, zero
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const unsigned long long z = draw_word(start, (row + pos_of(4 * w, h) + (n & 3)) * ng);
+          const unsigned long long z = draw_word(start + row + (unsigned long long)(16 * (w >> 1) + 4 * (w & 1)) * ng * DRAW_STEP);
           const unsigned lo = (unsigned)z, hi = (unsigned)(z >> 32);
           auto one = [&](int i, unsigned l, unsigned g) {
-            const unsigned f = n & 2 ? g : l;
-            const bool drop = (n & 1 ? f : f << 16) < thr << 16;
+            const bool drop = __builtin_amdgcn_perm(g, l, field) < thr << 16;
             p[i] = drop ? 0.f : x[i] * keep;
-            gone |= drop ? 1u << i : 0u;
+            if constexpr (!X3<E>) gone |= drop ? 1u << i : 0u;
           };
           one(4 * w, quad<0>(lo), quad<0>(hi));
           one(4 * w + 1, quad<1>(lo), quad<1>(hi));
@@ -177,18 +184,30 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
         }
       }
       // dv's product before dP's: P as an operand takes half the registers that dP will
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!EARLY) __builtin_amdgcn_sched_barrier(0);
       mul_rows<E, DP, 1, RB>(av, gs, rt, p, lane);
-      __builtin_amdgcn_sched_barrier(0);
-      f32x16 dp = mul_columns<E, DP, RB>(gs, rt, v, lane);
-      if (a.seed) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dp[i] = gone >> i & 1 ? 0.f : dp[i] * keep;
+      if constexpr (!EARLY) {
+        __builtin_amdgcn_sched_barrier(0);
+        dp = mul_columns<E, DP, RB>(gs, rt, v, lane);
       }
+      if constexpr (X3<E>) {
+        // P (Z dP - D) = (Z P) dP - P D needs no dropped bits, at sixteen registers that the 16-bit kernels lack
+        // (64 channels with dropout: 13 spills and 138-149 us against 133; fp32 at 96: 199 us against 217)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float g = x[i] * (dp[i] - rows[cur][32 * rt + pos_of(i, h)]);
-        x[i] = whole || x[i] > 0.f ? g : 0.f;                // (a masked entry: 0 whatever dO.v is)
+        for (int i = 0; i < 16; ++i) {
+          const float g = fmaf(p[i], dp[i], -(x[i] * rows[cur][32 * rt + pos_of(i, h)]));
+          x[i] = whole || x[i] > 0.f ? g : 0.f;
+        }
+      } else {
+        if (DROP && (EARLY || a.seed)) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dp[i] = gone >> i & 1 ? 0.f : dp[i] * keep;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float g = x[i] * (dp[i] - rows[cur][32 * rt + pos_of(i, h)]);
+          x[i] = whole || x[i] > 0.f ? g : 0.f;              // (a masked entry: 0 whatever dO.v is)
+        }
       }
       if (sc.cap) {
 #pragma unroll
@@ -221,8 +240,11 @@ template <typename E, int DP>
 static void go(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
   const int n_tiles = (a.Tk + NCOL - 1) / NCOL;
   const unsigned grid = (unsigned)grid_of((long long)a.B * a.G, 1, n_tiles);
-  if (sizeof(E) == 4 || a.dbias) hipLaunchKernelGGL((dkv_kernel<E, DP, true>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
-  else hipLaunchKernelGGL((dkv_kernel<E, DP, sizeof(E) == 4>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
+  const bool exact = sizeof(E) == 4 || a.dbias;
+  if (exact && a.seed) hipLaunchKernelGGL((dkv_kernel<E, DP, true, true>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
+  else if (exact) hipLaunchKernelGGL((dkv_kernel<E, DP, true, false>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
+  else if (a.seed) hipLaunchKernelGGL((dkv_kernel<E, DP, sizeof(E) == 4, true>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
+  else hipLaunchKernelGGL((dkv_kernel<E, DP, sizeof(E) == 4, false>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
 }
 template <typename E>
 static void pick(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {

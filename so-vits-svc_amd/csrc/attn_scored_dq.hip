@@ -19,7 +19,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
   __shared__ float bin_[4][2][NB];
   __shared__ float red[4];
   E* const tiles = (E*)tiles_;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, n = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, n = lane & 31;
   const Place at = place_of(blockIdx.x, a.B * a.G, a.H / a.G, n_tiles);
   if (at.group >= a.B * a.G) return;
   const int b = at.group / a.G, kvh = at.group % a.G, head = kvh * (a.H / a.G) + at.sub, t0 = at.tile * NCOL;
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
   unsigned thr = 0;
   float keep = 1.f;
   if (a.seed) {
-    draws = draw_start(a) + (unsigned long long)(bh * a.Tq + t) * (unsigned long long)((a.Tk + 3) >> 2) * 0xD1B54A32D192ED03ull;
+    draws = draw_start(a) + ((unsigned long long)(bh * a.Tq + t) * (unsigned long long)((a.Tk + 3) >> 2) + 2 * h) * DRAW_STEP;
     thr = (unsigned)rintf(a.p_drop * 65536.f);
     keep = 65536.f / (65536.f - (float)thr);
   }
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
       if (a.seed) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const unsigned long long z = draw_word(draws, (unsigned long long)((s0 + 32 * rt + pos_of(4 * w, h)) >> 2));
+          const unsigned long long z = draw_word(draws + draw_block(s0 + 32 * rt) + draw_group(w));
 #pragma unroll
           for (int j = 0; j < 4; ++j) dp[4 * w + j] = dropped(z, j, thr) ? 0.f : dp[4 * w + j] * keep;
         }

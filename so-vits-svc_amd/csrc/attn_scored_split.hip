@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256, DP > (sizeof(E) == 4 ? 64 : 96) ? 1 : 2) void 
   // (two workgroups of 128 channels take the CU's LDS to the byte: the waves' maxima and sums go where their tiles end)
   auto ms = [&](int w) { return (float*)(lds_ + w * WAVE + DP * 128); };
   auto ls = [&](int w) { return (float*)(lds_ + w * WAVE + DP * 128) + 32; };
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, n = lane & 31, rep = a.H / a.G;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, n = lane & 31, rep = a.H / a.G;
   const int part = blockIdx.x % sp.parts, blk = blockIdx.x / sp.parts % sp.blocks, bg = blockIdx.x / (sp.parts * sp.blocks);
   const int b = bg / a.G, kvh = bg % a.G, col = blk * 32 + n;
   const bool in = col < sp.cols;
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256, DP > (sizeof(E) == 4 ? 64 : 96) ? 1 : 2) void 
   unsigned long long draws = 0;
   unsigned thr = 0;
   if (a.seed) {
-    draws = draw_start(a) + (unsigned long long)(((long long)b * a.H + head) * a.Tq + t) * (unsigned long long)((a.Tk + 3) >> 2) * 0xD1B54A32D192ED03ull;
+    draws = draw_start(a) + ((unsigned long long)(((long long)b * a.H + head) * a.Tq + t) * (unsigned long long)((a.Tk + 3) >> 2) + 2 * h) * DRAW_STEP;
     thr = (unsigned)rintf(a.p_drop * 65536.f);
   }
   f32x16 acc[DP / 32];
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256, DP > (sizeof(E) == 4 ? 64 : 96) ? 1 : 2) void 
     if (a.seed) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const unsigned long long z = draw_word(draws, (unsigned long long)((s0 + pos_of(4 * w, h)) >> 2));
+        const unsigned long long z = draw_word(draws + draw_block(s0) + draw_group(w));
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[4 * w + j] = dropped(z, j, thr) ? 0.f : s[4 * w + j];
       }
