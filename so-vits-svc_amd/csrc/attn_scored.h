@@ -168,20 +168,27 @@ template <typename E, int DP, int RB = 128, int TH = 256> struct Pre { uint4 v[D
 
 template <typename E, int DP, int RB = 128, int TH = 256>
 struct Source {                         // one head's matrix as this thread sees it
-  const E *row, *last;                  // its row of step 0 and of the last step (whose rows may lie behind dk: the nearest row stands for them)
+  static constexpr int CH = Tile<E, RB, TH>::CH, RS = Tile<E, RB, TH>::RS, S = DP / RS, V = Tile<E, RB>::V;
+  static constexpr int TAIL = RS < 32 ? 32 / RS : 1;      // dk > DP - 32: the steps whose rows may lie behind dk (the last row stands for them, read and not used)
+  static_assert(TAIL <= S, "");
+  const E *row, *tail[TAIL];            // its rows of step 0 and of the last steps
   long long step;                       // elements between steps
   int T;                                // positions that exist
-  bool pad;                             // its last row lies behind dk
-  static constexpr int CH = Tile<E, RB, TH>::CH, RS = Tile<E, RB, TH>::RS, S = DP / RS, V = Tile<E, RB>::V;
+  int pad;                              // bit j: its row of the j-th of the last steps lies behind dk
   __device__ __forceinline__ void set(const E* x, long long cs, int dk, int T_, int tid) {
-    const int d = tid / CH, dl = d + DP - RS;
-    row = x + (long long)d * cs;
-    last = x + (long long)min(dl, dk - 1) * cs;
+    const int d = tid / CH;
+    row = x + (long long)min(d, dk - 1) * cs;
     step = RS * cs;
     T = T_;
-    pad = dl >= dk;
-    if (DP == RS) row = last;
+    pad = 0;
+#pragma unroll
+    for (int j = 0; j < TAIL; ++j) {
+      const int dl = d + (S - TAIL + j) * RS;
+      tail[j] = x + (long long)min(dl, dk - 1) * cs;
+      pad |= dl >= dk ? 1 << j : 0;
+    }
   }
+  __device__ __forceinline__ const E* at(int i) const { return i >= S - TAIL ? tail[i - (S - TAIL)] : row + i * step; }
   // Sixteen bytes a step, from the chunk's place or, at the row's end, from the last place that has sixteen: no branch, because a branch around loads makes
   // the compiler wait for them where its sides meet again.  (Rows of fewer than sixteen bytes are read by `commit`.)
   __device__ __forceinline__ void fetch(Pre<E, DP, RB, TH>& f, int p0, int tid) const {
@@ -189,7 +196,7 @@ struct Source {                         // one head's matrix as this thread sees
     const int p = min(p0 + (tid & (CH - 1)) * V, T - V);
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      const U128 u = *(const U128*)((i == S - 1 ? last : row + i * step) + p);
+      const U128 u = *(const U128*)(at(i) + p);
       f.v[i] = make_uint4(u.x, u.y, u.z, u.w);
     }
   }
@@ -201,7 +208,7 @@ struct Source {                         // one head's matrix as this thread sees
         for (int i = 0; i < S; ++i) {
           union { uint4 u; E e[V]; } x;
           x.u = make_uint4(0, 0, 0, 0);
-          const E* r = i == S - 1 ? last : row + i * step;
+          const E* r = at(i);
 #pragma unroll
           for (int e = 0; e < V; ++e)
             if (p + e < T) x.e[e] = r[p + e];
@@ -228,7 +235,11 @@ struct Source {                         // one head's matrix as this thread sees
 #pragma unroll
       for (int i = 0; i < S; ++i) f.v[i] = make_uint4(f.v[i].x & k[0], f.v[i].y & k[1], f.v[i].z & k[2], f.v[i].w & k[3]);
     }
-    if (pad) f.v[S - 1] = make_uint4(0, 0, 0, 0);
+    if (pad) {
+#pragma unroll
+      for (int j = 0; j < TAIL; ++j)
+        if (TAIL == 1 || pad >> j & 1) f.v[S - TAIL + j] = make_uint4(0, 0, 0, 0);
+    }
     if constexpr (X3<E>) {
       static_assert(RB == 128, "32 positions");
 #pragma unroll

@@ -500,7 +500,9 @@ int check(const svc_dropout_add_layernorm_t* a, bool backward) {
   SVC_REQUIRE(!a->seed || (a->p >= 0.f && a->p < 1.f), "dropout_add_layernorm: rate %g (0 <= p < 1)", a->p);
   SVC_REQUIRE(a->eps > 0.f, "dropout_add_layernorm: eps %g", a->eps);
   if (a->B == 0 || a->T == 0) return SVC_OK;
-  SVC_REQUIRE((long long)a->B * svc::cdiv(a->T, 8) < (1LL << 31) && a->C < (1 << 30), "dropout_add_layernorm: B=%d C=%d T=%d", a->B, a->C, a->T);
+  // (a launch has fewer than 2^32 threads: 512 for 16 columns, 1024 for 16 channels' sums)
+  SVC_REQUIRE((long long)a->B * svc::cdiv(a->T, 16) < (1LL << 23) && a->C < (1 << 25), "dropout_add_layernorm: B=%d C=%d T=%d (built for 2^27 columns, 2^25 channels)",
+              a->B, a->C, a->T);
   SVC_REQUIRE(a->x && a->gamma && a->beta, "dropout_add_layernorm: x, gamma, beta");
   if (!backward) {
     SVC_REQUIRE(a->y && !a->mean == !a->rstd, "dropout_add_layernorm_fwd: y, and mean with rstd");

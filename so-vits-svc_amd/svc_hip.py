@@ -2075,6 +2075,8 @@ def _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, pr
     if n_heads < 1 or Cq % n_heads or Cq == 0:
         raise SvcError(f"{what}: {Cq} channels do not split into {n_heads} heads")
     dk = Cq // n_heads
+    if max(B, Cq, Tk, Tq, k.shape[1]) >= 1 << 30:      # (the struct's fields are 32-bit)
+        raise SvcError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}; built for sizes below 2^30")
     if k.shape != v.shape or k.shape[0] != B or k.shape[1] % dk or k.shape[1] == 0 or n_heads % (k.shape[1] // dk):
         raise SvcError(f"{what}: q {tuple(q.shape)} in {n_heads} heads of {dk}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     if dk > 128:
@@ -2087,7 +2089,7 @@ def _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, pr
     if not a.scale > 0.0:
         raise SvcError(f"{what}: scale {scale}")
     a.softcap, a.causal = softcap or 0.0, 1 if causal else 0
-    a.window = -1 if window is None else window
+    a.window = -1 if window is None else min(window, Tk)      # (a position is below Tk: a wider window is none)
     if window is not None and window < 0:
         raise SvcError(f"{what}: window {window}")
     if offset is None:
@@ -2101,7 +2103,7 @@ def _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, pr
     if lengths is not None:
         a.lengths = _side(what, "lengths", lengths, (B,), torch.int32, dev)
     if docs is not None:
-        if docs.dim() != 2 or docs.shape[1] < 2:
+        if docs.dim() != 2 or not 2 <= docs.shape[1] <= 1 << 30:
             raise SvcError(f"{what}: docs are boundaries [B, N + 1]; got {tuple(docs.shape)}")
         a.n_docs = docs.shape[1] - 1
         a.docs = _side(what, "docs", docs, (B, a.n_docs + 1), torch.int32, dev)
@@ -2112,6 +2114,8 @@ def _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, pr
     if bias is not None:
         if bias.dim() != 2 or bias.shape[0] not in (1, n_heads) or bias.shape[1] % 2 == 0:
             raise SvcError(f"{what}: bias [{n_heads} or 1, 2 W + 1]; got {tuple(bias.shape)}")
+        if bias.shape[1] >> 25:
+            raise SvcError(f"{what}: bias {tuple(bias.shape)}; built for W < 2^24")
         a.bias_heads, a.bias_w = bias.shape[0], bias.shape[1] // 2
         a.bias = _side(what, "bias", bias, bias.shape, torch.float32, dev)
     if p_drop and _drop_args(what, a, draw, p_drop, dev):
@@ -2127,7 +2131,7 @@ def attention_scored(q, k, v, n_heads, *, bias=None, softcap=0.0, scale=None, ca
     Queries are positions `offset` .. `offset + Tq - 1` of the key axis (int, or int32 [B]; default: the last Tq).  `lengths` int32 [B]: the
     valid positions of each item.  `docs` int32 [B, N + 1]: boundaries of packed documents.  `causal`, with `prefix` (int32 [B], or [B, N] with
     documents) a bidirectional front; `window`: |s - p| <= window.  `softcap`: scores capped to softcap * tanh(score / softcap).  `bias` fp32
-    [H or 1, 2 W + 1]: added by distance, clamped to +-W.  A query that sees no key gives 0."""
+    [H or 1, 2 W + 1]: added by distance, clamped to +-W.  A query that sees no key gives 0.  `out` may be a view; it shares no memory with the inputs."""
     a, dev = _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, None, 0.0)
     if out is None:
         out = torch.empty(q.shape, device=dev, dtype=q.dtype)
@@ -2135,6 +2139,8 @@ def attention_scored(q, k, v, n_heads, *, bias=None, softcap=0.0, scale=None, ca
         _typed("attention_scored", q, out)
         if out.shape != q.shape:
             raise SvcError(f"attention_scored: out {tuple(out.shape)} for q {tuple(q.shape)}")
+        if out.numel() and (out.data_ptr() in (a.q, a.k, a.v) or 0 in [st for st, n in zip(out.stride(), out.shape) if n > 1]):
+            raise SvcError("attention_scored: out shares memory with an input, or its elements with each other")
     a.out = out.data_ptr()
     a.o_bs, a.o_cs = _bct_strides(out)
     ws = _scored_ws(a, 0, dev)
@@ -2216,8 +2222,8 @@ def _junction_args(x, r, gamma, beta, mask, draw, p, eps):
         raise SvcError(f"{what}: x {tuple(x.shape)}, r {None if r is None else tuple(r.shape)}; two [B, C, T] tensors of one shape")
     a = DropoutAddLayernorm()
     B, Cc, T = x.shape
-    if B > 65535:
-        raise SvcError(f"{what}: batch of {B}; built for up to 65535")
+    if B > 65535 or Cc >= 1 << 25 or B * ((T + 15) // 16) >= 1 << 23:
+        raise SvcError(f"{what}: {tuple(x.shape)}; built for B < 2^16, C < 2^25 and B ceil(T / 16) < 2^23")
     a.gamma, a.beta = _side(what, "gamma", gamma, (Cc,), torch.float32, dev), _side(what, "beta", beta, (Cc,), torch.float32, dev)
     if mask is not None:
         if mask.dim() == 3 and mask.shape[1] == 1:

@@ -182,6 +182,22 @@ def test_offsets_out_of_every_range(dev):
 
 
 @pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("Tq", [1, 5, 70])
+@pytest.mark.parametrize("dk", [1, 7, 9, 20, 33, 47, 65, 81, 97, 113])
+def test_a_head_reads_its_own_channels_only(dev, dt, Tq, dk):
+    """Head sizes between the built ones: the next head's channels (nan here) stand where a tile's rows behind dk would be."""
+    import svc_hip as S
+    g = torch.Generator().manual_seed(dk + Tq)
+    q, k, v = (torch.randn(1, 2 * dk, T, generator=g).to(TYPES[dt]).to(dev) for T in (Tq, 90, 90))
+    want = S.attention_scored(*(x[:, :dk].contiguous() for x in (q, k, v)), 1, causal=True)
+    for x in (q, k, v):
+        x[:, dk:] = float("nan")
+    got = S.attention_scored(q, k, v, 2, causal=True)
+    assert torch.equal(got[:, :dk], want)
+    assert torch.isnan(got[:, dk:]).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
 def test_views_and_alignment(dev, dt):
     """q, k, v as channel slices of one projection and as time slices at odd starts, channels in reverse order of a larger tensor; out as a view whose
     surroundings stay as they were."""

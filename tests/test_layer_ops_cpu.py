@@ -55,7 +55,8 @@ BAD = [dict(dtype=3), dict(dtype=-1), dict(B=-1), dict(Tq=9), dict(Tq=-1), dict(
        dict(offset=1), dict(offset=-1), dict(window=-2), dict(n_docs=2), dict(n_docs=-1), dict(prefix=4096), dict(prefix=4096, causal=1, window=3),
        dict(bias=4096, bias_heads=2), dict(bias=4096, bias_heads=4, bias_w=-1), dict(softcap=-1.0), dict(softcap=float("inf")),
        dict(softcap=float("nan")), dict(scale=float("nan")), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(seed=4096, p_drop=1.0), dict(seed=4096, p_drop=-0.1), dict(seed=4096, p_drop=float("nan")),
-       dict(q=None), dict(k=None), dict(v=None), dict(B=1 << 30, Tk=1 << 20)]
+       dict(q=None), dict(k=None), dict(v=None), dict(B=1 << 30, Tk=1 << 20), dict(B=5 << 18, Tk=1, Tq=1), dict(bias=4096, bias_heads=1, bias_w=1 << 24),
+       dict(bias=4096, bias_heads=65536, H=65536)]
 
 
 @pytest.mark.parametrize("bad", BAD, ids=lambda d: ",".join(f"{k}={v}" for k, v in d.items()))
@@ -93,7 +94,7 @@ def _junction(**kw):
     return a
 
 
-@pytest.mark.parametrize("bad", [dict(dtype=3), dict(B=-1), dict(B=65536), dict(C=0), dict(T=-1), dict(eps=0.0), dict(eps=float("nan")), dict(x=None),
+@pytest.mark.parametrize("bad", [dict(dtype=3), dict(B=-1), dict(B=65536), dict(C=0), dict(T=-1), dict(C=1 << 25), dict(T=1 << 26), dict(eps=0.0), dict(eps=float("nan")), dict(x=None),
                                  dict(gamma=None), dict(beta=None), dict(seed=4096, p=1.0), dict(seed=4096, p=-0.5), dict(seed=4096, p=float("nan"))])
 def test_junction_refuses(bad):
     import svc_hip as S
