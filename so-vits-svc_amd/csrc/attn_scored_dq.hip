@@ -1,4 +1,9 @@
 // attn_scored_dq.hip — svc_attn_scored_bwd's walk over the keys: dq and the bias gradient.
+//
+// P = exp2(x - lse) again from q and k, dP = Z (dO.v), dS = P (dP - D): three products, with q's and dO's columns in registers throughout.  The vector
+// unit bounds it (scores as in the forward, and the mask, D and cap factors of dS).  Measured: bf16, 128 channels, 4 x 16 heads, 4096 x 4096 causal with a
+// cap 575 us = 720 TFLOP/s of its three products; bf16, 64 channels, 9 documents in 4099 with bias and dropout 71 us; fp16, window of 128 in 1501 with
+// the bias's gradient 95 us; fp32, 96 channels, 16 ragged items of up to 790 131 us.
 #include "attn_scored.h"
 
 namespace attn {
@@ -78,7 +83,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
   // Bias gradient.  A 32 x 32 block's entries of one distance lie on a diagonal: register j of eight (neighbouring positions) and lane n belong to
   // distance j - n.  The eight are summed along their diagonals in registers by shifting lanes one step per register, downwards for the lanes n >= j
   // and upwards for the others (neither crosses into the other half of the wave: what would is zero); the two results, 32 and 7 distances, are added to
-  // the half's own bins in LDS, 4 additions a block instead of 16 (LDS additions of every register held the kernel: train_window_fp16 267 us).  The
+  // the half's own bins in LDS, 4 additions a block instead of 16 (LDS additions of every register held the kernel: fp16, window of 128 in 1501: 267 us for 96).  The
   // lanes of one addition never meet, nor do waves, so the order is fixed.  As the tiles advance by N keys, a wave's first N bins are complete after
   // each tile and leave; the last 32 stay.  Distances at or beyond +-bias_w share the table's end entries and are summed in registers.
   const int W = a.bias_w;

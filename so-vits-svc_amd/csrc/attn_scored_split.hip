@@ -4,6 +4,8 @@
 // that shared key heads are read once — and one of `parts` equal parts of the keys they see; its four waves take tiles of it in turn, each through LDS
 // of its own, with no barrier until their results are joined.  Bandwidth is the bound: the next tile's loads (16 KB a wave at 128 channels) are in
 // flight while a tile is worked on.  With more than one part the partial maxima, sums and outputs go through the workspace and a second launch.
+// Measured: 16 streams, 16 query and 4 key heads of 128 channels, caches of 8191 keys of different fill, bf16: 54 us = 3.8 TB/s, and 6.6 us to join the
+// parts; 2 heads of 96 channels, 862 keys, fp32: 19 + 4 us, latency: two launches, and a wave's two tiles one after the other.
 #include "attn_scored.h"
 
 namespace attn {
@@ -235,7 +237,8 @@ __global__ __launch_bounds__(256) void join_kernel(svc_attn_scored_t a, Split sp
 }
 
 // Few queries (up to 64: fwd_kernel's workgroups of 128 would stand half empty), parts so that there are about two workgroups a CU, each wave with two
-// tiles at least.
+// tiles at least.  This way against fwd_kernel's: one query over 862 keys fp32 24 us for 105, one for each of 16 streams over 8191 keys 81 for 279 (64
+// since), 37 queries over 1500 keys with a window of 200 15.5 for 15.7: even where the columns fill the workgroup.
 Split split_of(const svc_attn_scored_t& a) {
   Split p;
   p.cols = a.H / a.G * a.Tq;

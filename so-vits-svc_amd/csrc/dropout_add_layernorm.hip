@@ -3,6 +3,11 @@
 //
 // The backward keeps nothing but mean and rstd: h = r + dropout(x) is recomputed from x, r and the counter draws, which moves the same bytes as
 // storing h would (one write and one read against two reads in place of one) and takes no memory.
+//
+// Measured, 32 x 768 x 1499 bf16 with dropout: forward 91 us (221 MB, 2.4 TB/s), backward 188 us (368 MB, 2.0 TB/s).  The draws are the bound: two 64-bit
+// multiplications an element, 6 quarter-rate instructions of about 40; with the rest of the arithmetic 72 of the forward's us and 86 of the backward's are
+// vector instructions, and a tile's loads, sums and stores stand one behind the other in each workgroup.  16 x 192 x 790 fp32: 13 and 19 us, a tile's
+// own length; 8 x 1001 x 2047 fp16 without dropout: 42 and 69 us (98 and 131 MB).
 #include "common.h"
 
 namespace {
@@ -438,7 +443,8 @@ __global__ __launch_bounds__(1024) void junction_param_kernel(const float* __res
 
 // How a launch is cut.  LPR = 4: 16 time steps a workgroup, up to 1024 channels in at most 128 registers a thread, which leaves room for a second workgroup
 // on the CU: one loads while the other draws, sums and stores.  LPR = 2: 8 steps, for tensors of so few columns that 16-step tiles would leave
-// most CUs without one.  NR: channels of a thread, the smallest built number that covers C; none: the kernels that read the tensors again.
+// most CUs without one (1 x 192 x 862 fp32: 6.2 us for 7.9 with 16; 16 x 192 x 790: 19 and 23 us with 8 for 13 and 19 with 16).  NR: channels of a
+// thread, the smallest built number that covers C; none: the kernels that read the tensors again (32 x 768 x 1499 bf16: 265 and 360 us for 91 and 188).
 struct Plan {
   int lpr, nr, tiles_t, blocks;
   long long n_tiles;
