@@ -41,12 +41,24 @@ struct x3_t {
 };
 template <typename E> constexpr bool X3 = __is_same(E, x3_t);
 constexpr int X3_PITCH = 80;            // bytes of a plane's row of 32 positions: 64 + 16
-__device__ __forceinline__ void split3(float x, bf16_t& a, bf16_t& b, bf16_t& c) {
-  a = (bf16_t)x;
-  const float r = x - (float)a;
-  const float s = fabsf(r) < INFINITY ? r : 0.f;      // (an infinity or nan is its first part alone)
-  b = (bf16_t)s;
-  c = (bf16_t)(s - (float)b);
+// Two values rounded to bf16 in one word, and what the rounding left of them.  (One value at a time the compiler converts each twice, once for its word.)
+__device__ __forceinline__ unsigned pack2(float x, float y) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){x, y}, b2));
+}
+__device__ __forceinline__ void rest2(float& x, float& y, unsigned u) {
+  x -= __builtin_bit_cast(float, u << 16);
+  y -= __builtin_bit_cast(float, u & 0xffff0000u);
+}
+__device__ __forceinline__ void split3(float x, float y, unsigned& a, unsigned& b, unsigned& c) {
+  a = pack2(x, y);
+  rest2(x, y, a);
+  x = fabsf(x) < INFINITY ? x : 0.f;      // (an infinity or nan is its first part alone)
+  y = fabsf(y) < INFINITY ? y : 0.f;
+  b = pack2(x, y);
+  rest2(x, y, b);
+  c = pack2(x, y);
 }
 
 // A staged tile: rows of RB bytes of positions and 16 bytes more, which spreads both operand reads over all banks.  128-byte rows (64 positions of a 16-bit
@@ -244,21 +256,14 @@ struct Source {                         // one head's matrix as this thread sees
       static_assert(RB == 128, "32 positions");
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        typedef bf16_t b4 __attribute__((ext_vector_type(4)));
         const f32x4 x = __builtin_bit_cast(f32x4, f.v[i]);
-        b4 a, b, c;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          bf16_t u, v, w;
-          split3(x[e], u, v, w);
-          a[e] = u;
-          b[e] = v;
-          c[e] = w;
-        }
+        uint2 u, v, w;
+        split3(x[0], x[1], u.x, v.x, w.x);
+        split3(x[2], x[3], u.y, v.y, w.y);
         char* o = (char*)lds + (tid / CH + i * RS) * X3_PITCH + (tid & (CH - 1)) * 8;
-        *(b4*)o = a;
-        *(b4*)(o + DP * X3_PITCH) = b;
-        *(b4*)(o + 2 * DP * X3_PITCH) = c;
+        *(uint2*)o = u;
+        *(uint2*)(o + DP * X3_PITCH) = v;
+        *(uint2*)(o + 2 * DP * X3_PITCH) = w;
       }
       return;
     }
@@ -371,15 +376,9 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
   const E* p = lds + (lane & 31) * Tile<E, RB>::P + 32 * rt + 8 * h;
   if constexpr (X3<E>) {
     const char* q = (const char*)lds + (lane & 31) * X3_PITCH + 2 * (32 * rt + 8 * h);
-    bf16x8 b[2][3];
+    union { unsigned u[4]; bf16x8 v; } b[2][3];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      bf16_t u, v, z;
-      split3(w[e], u, v, z);
-      b[e >> 3][0][e & 7] = u;
-      b[e >> 3][1][e & 7] = v;
-      b[e >> 3][2][e & 7] = z;
-    }
+    for (int e = 0; e < 8; ++e) split3(w[2 * e], w[2 * e + 1], b[e >> 2][0].u[e & 3], b[e >> 2][1].u[e & 3], b[e >> 2][2].u[e & 3]);
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) {
       f32x16 small;
@@ -390,7 +389,7 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
         bf16x8 x[3];
 #pragma unroll
         for (int k = 0; k < 3; ++k) x[k] = *(const bf16x8*)(q + (k * DP + 32 * dt) * X3_PITCH + 32 * ks);
-        mfma6(x, b[ks][0], b[ks][1], b[ks][2], out[dt], small);
+        mfma6(x, b[ks][0].v, b[ks][1].v, b[ks][2].v, out[dt], small);
       }
       out[dt] += small;
       __builtin_amdgcn_sched_barrier(0);
@@ -407,21 +406,28 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
   } else {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      typename Frag<E>::V b[OPS];
+      union { unsigned u[4]; typename Frag<E>::V v; } b[OPS];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float rest = w[8 * ks + e];
+      for (int e = 0; e < 4; ++e) {
+        float x = w[8 * ks + 2 * e], y = w[8 * ks + 2 * e + 1];
 #pragma unroll
         for (int o = 0; o < OPS; ++o) {
-          b[o][e] = (E)rest;
-          rest -= (float)b[o][e];
+          if constexpr (__is_same(E, bf16_t)) {
+            b[o].u[e] = pack2(x, y);
+            if (o + 1 < OPS) rest2(x, y, b[o].u[e]);
+          } else {
+            b[o].v[2 * e] = (E)x;
+            b[o].v[2 * e + 1] = (E)y;
+            x -= (float)b[o].v[2 * e];
+            y -= (float)b[o].v[2 * e + 1];
+          }
         }
       }
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
         const typename Frag<E>::V v = *(const typename Frag<E>::V*)(p + 32 * dt * Tile<E, RB>::P + 16 * ks);
 #pragma unroll
-        for (int o = 0; o < OPS; ++o) out[dt] = mfma(v, b[o], out[dt]);
+        for (int o = 0; o < OPS; ++o) out[dt] = mfma(v, b[o].v, out[dt]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
