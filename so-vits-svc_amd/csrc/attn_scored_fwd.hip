@@ -6,8 +6,8 @@
 // unit is the bound, not the matrix unit: 16 scores a lane cost 32 to 48 transcendental cycles and 8 to 30 ordinary instructions each (cap, bias, mask,
 // draws), the products 512 to 1024 cycles for all; two waves a SIMD overlap the two.  128 queries a workgroup share every k and v tile through LDS; a
 // tile's loads are in flight while the one before is worked on.  Measured (kernel alone): bf16, 128 channels, 4 x 16 heads, 4096 x 4096 causal with a
-// cap 520 us = 530 TFLOP/s; a call of 2049 x 2049 with a prefix 146 us = 500; bf16, 64 channels, 9 documents in 4099 with bias and dropout 64 us; fp16, window
-// of 128 in 1501 58 us; fp32, 96 channels, 16 ragged items of up to 790 with dropout 94 us.
+// cap 505 us = 545 TFLOP/s; a call of 2049 x 2049 with a prefix 145 us = 500; bf16, 64 channels, 9 documents in 4099 with bias and dropout 60 us; fp16, window
+// of 128 in 1501 58 us; fp32, 96 channels, 16 ragged items of up to 790 with dropout 92 us.
 #include "attn_scored.h"
 
 namespace attn {
