@@ -61,17 +61,22 @@ __device__ __forceinline__ void split3(float x, float y, unsigned& a, unsigned& 
   c = pack2(x, y);
 }
 
-// A staged tile: rows of RB bytes of positions and 16 bytes more, which spreads both operand reads over all banks.  128-byte rows (64 positions of a 16-bit
-// type, 32 of fp32); 64-byte rows for the backward at 128 channels in 16 bits, whose accumulators leave no registers for a longer tile's loads.
+// A staged tile: rows of RB bytes of positions.  128-byte rows (64 positions of a 16-bit type, 32 of fp32); 64-byte rows for the backward at 128
+// channels in 16 bits, whose accumulators leave no registers for a longer tile's loads.  fp32's rows have 16 bytes more, which spreads their reads over the
+// banks.  16-bit types' rows are not padded: chunk c (16 bytes) of row d lies at c ^ turn(d), so that the four rows x 64 bytes of a transposing
+// read, and the sixteen rows x 16 bytes of an ordinary one, each fall on all 64 banks once (rows padded by 16 bytes: 6 to 17 % of the cycles in conflicts,
+// dq at 128 channels 575 us for 560).
 template <typename E, int RB = 128, int TH = 256> struct Tile {
   static constexpr int N = RB / (int)sizeof(E);
   static constexpr int RT = N / 32;     // 32-row accumulators a tile feeds
-  static constexpr int PITCH = RB + 16;
+  static constexpr int PITCH = RB + (sizeof(E) == 2 ? 0 : 16);
   static constexpr int P = PITCH / (int)sizeof(E);
   static constexpr int V = 16 / (int)sizeof(E);     // positions of a 16-byte chunk
   static constexpr int CH = RB / 16;                // chunks (lanes) of a row
   static constexpr int RS = TH / CH;                // rows that TH threads stage in one step
 };
+
+template <int RB> __device__ __forceinline__ int turn(int d) { return RB == 128 ? (d & 2) << 1 | (d >> 2 & 3) : d >> 2 & 3; }
 
 template <typename E, int DP, int RB = 128> struct Staged {
   static constexpr int SIZE = X3<E> ? 3 * DP * X3_PITCH / 4 : DP * Tile<E, RB>::P;     // elements of E from one staged matrix to the next
@@ -268,19 +273,24 @@ struct Source {                         // one head's matrix as this thread sees
       return;
     }
     constexpr int PITCH = Tile<E, RB>::PITCH;
-    char* o = (char*)lds + tid / CH * PITCH + (tid & (CH - 1)) * 16;
+    // (a step is a multiple of 16 rows, or fp32's: the turn is the same in all)
+    static_assert(sizeof(E) == 4 || RS % 16 == 0, "");
+    const int d0 = tid / CH, chunk = tid & (CH - 1);
+    char* o = (char*)lds + d0 * PITCH + (sizeof(E) == 2 ? chunk ^ turn<RB>(d0) : chunk) * 16;
 #pragma unroll
     for (int i = 0; i < S; ++i) *(uint4*)(o + i * RS * PITCH) = f.v[i];
   }
 };
 
-// Four rows (d) of 16 columns each, transposed: lane i of 16 gets column i's four values.
-template <typename E> __device__ __forceinline__ typename Frag<E>::V read_transposed(const void* p, int four_rows) {
+// Four rows (d) of 16 columns each, transposed: lane i of 16 gets column i's four values; and the four rows behind them.
+template <typename E> __device__ __forceinline__ typename Frag<E>::V read_transposed(const void* p, const void* p4) {
   typedef __attribute__((address_space(3))) s16x4 lds4;
   const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)((const char*)p + four_rows));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p4);
   return __builtin_bit_cast(typename Frag<E>::V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
+// byte of (row d, column c) in a 16-bit type's tile
+template <int RB> __device__ __forceinline__ int byte_of(int d, int c) { return d * RB + ((c >> 3 ^ turn<RB>(d)) << 4) + (c & 7) * 2; }
 
 // Columns 32 sub .. 32 sub + 31 of a staged tile as a right operand that reduces over d.
 template <typename E, int DP, int RB = 128>
@@ -291,15 +301,16 @@ __device__ __forceinline__ void read_columns(typename Frag<E>::template Head<DP>
 #pragma unroll
     for (int k = 0; k < 3; ++k)
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i) f.v[k][i] = read_transposed<E>(p + (k * DP + 16 * i) * X3_PITCH, 4 * X3_PITCH);
+      for (int i = 0; i < DP / 16; ++i) f.v[k][i] = read_transposed<E>(p + (k * DP + 16 * i) * X3_PITCH, p + (k * DP + 16 * i + 4) * X3_PITCH);
   } else if constexpr (sizeof(E) == 4) {
     const float* p = lds + h * Tile<E, RB>::P + 32 * sub + (lane & 31);
 #pragma unroll
     for (int i = 0; i < DP / 2; ++i) f.v[i] = p[2 * i * Tile<E, RB>::P];
   } else {
-    const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E, RB>::P + 32 * sub + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+    const int d = 8 * h + (i16 >> 2), c = 32 * sub + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+    const char *p = (const char*)lds + byte_of<RB>(d, c), *p4 = (const char*)lds + byte_of<RB>(d + 4, c);
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) f.v[i] = read_transposed<E>(p + 16 * i * Tile<E, RB>::P, 4 * Tile<E, RB>::PITCH);
+    for (int i = 0; i < DP / 16; ++i) f.v[i] = read_transposed<E>(p + 16 * i * RB, p4 + 16 * i * RB);
   }
 }
 
@@ -342,7 +353,7 @@ __device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typena
     for (int i = 0; i < DP / 16; ++i) {
       bf16x8 x[3];
 #pragma unroll
-      for (int k = 0; k < 3; ++k) x[k] = read_transposed<E>(p + (k * DP + 16 * i) * X3_PITCH, 4 * X3_PITCH);
+      for (int k = 0; k < 3; ++k) x[k] = read_transposed<E>(p + (k * DP + 16 * i) * X3_PITCH, p + (k * DP + 16 * i + 4) * X3_PITCH);
       mfma6(x, f.v[0][i], f.v[1][i], f.v[2][i], acc, other);
       if (i & 1) __builtin_amdgcn_sched_barrier(0);
     }
@@ -358,10 +369,14 @@ __device__ __forceinline__ f32x16 mul_columns(const E* lds, int rt, const typena
     }
     acc = acc + other;
   } else {
-    const E* p = lds + (8 * h + (i16 >> 2)) * Tile<E, RB>::P + 32 * rt + 16 * ((lane >> 4) & 1) + c4;
+    // (columns 32 rt further are the byte's bit 6, the four rows behind are bit 4 and 4 rows: worked out here, from one register that stays)
+    int at = byte_of<RB>(8 * h + (i16 >> 2), 16 * ((lane >> 4) & 1) + c4);
+    asm volatile("" : "+v"(at));
+    at ^= 64 * rt;
+    const char *p = (const char*)lds + at, *p4 = (const char*)lds + (at ^ 16) + 4 * RB;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
-      acc = mfma(read_transposed<E>(p + 16 * i * Tile<E, RB>::P, 4 * Tile<E, RB>::PITCH), f.v[i], acc);
+      acc = mfma(read_transposed<E>(p + 16 * i * RB, p4 + 16 * i * RB), f.v[i], acc);
       if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -406,6 +421,9 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
   } else {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
+      int at = byte_of<RB>(lane & 31, 8 * h);
+      asm volatile("" : "+v"(at));
+      const char* const row = (const char*)lds + (at ^ (64 * rt + 32 * ks));
       union { unsigned u[4]; typename Frag<E>::V v; } b[OPS];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -425,7 +443,7 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
       }
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
-        const typename Frag<E>::V v = *(const typename Frag<E>::V*)(p + 32 * dt * Tile<E, RB>::P + 16 * ks);
+        const typename Frag<E>::V v = *(const typename Frag<E>::V*)(row + 32 * dt * RB);
 #pragma unroll
         for (int o = 0; o < OPS; ++o) out[dt] = mfma(v, b[o].v, out[dt]);
       }

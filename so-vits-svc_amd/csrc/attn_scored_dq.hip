@@ -2,7 +2,7 @@
 //
 // P = exp2(x - lse) again from q and k, dP = Z (dO.v), dS = P (dP - D): three products, with q's and dO's columns in registers throughout.  The vector
 // unit bounds it (scores as in the forward, and the mask, D and cap factors of dS).  Measured: bf16, 128 channels, 4 x 16 heads, 4096 x 4096 causal with a
-// cap 575 us = 720 TFLOP/s of its three products; bf16, 64 channels, 9 documents in 4099 with bias and dropout 71 us; fp16, window of 128 in 1501 with
+// cap 560 us = 735 TFLOP/s of its three products; bf16, 64 channels, 9 documents in 4099 with bias and dropout 71 us; fp16, window of 128 in 1501 with
 // the bias's gradient 95 us; fp32, 96 channels, 16 ragged items of up to 790 131 us.
 #include "attn_scored.h"
 

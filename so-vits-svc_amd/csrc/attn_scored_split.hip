@@ -19,10 +19,10 @@ __global__ __launch_bounds__(256, DP > (sizeof(E) == 4 ? 64 : 96) ? 1 : 2) void 
   typedef Tile<E, RB, 64> TL;
   constexpr int N = TL::N;
   static_assert(TL::RT == 1, "a wave's tile is 32 keys");
-  constexpr int WAVE = 2 * DP * TL::PITCH;                        // bytes of a wave's k and v tiles; its output, DP x 32 floats, fits
-  static_assert(WAVE >= DP * 32 * 4 + 256, "");
+  // bytes of a wave: its k and v tiles, in whose place its output, DP x 32 floats, and its maxima and sums come
+  constexpr int WAVE = 2 * DP * TL::PITCH > DP * 128 + 256 ? 2 * DP * TL::PITCH : DP * 128 + 256;
   __shared__ __align__(16) char lds_[4 * WAVE];
-  // (two workgroups of 128 channels take the CU's LDS to the byte: the waves' maxima and sums go where their tiles end)
+  // (the waves' maxima and sums go behind their outputs)
   auto ms = [&](int w) { return (float*)(lds_ + w * WAVE + DP * 128); };
   auto ls = [&](int w) { return (float*)(lds_ + w * WAVE + DP * 128) + 32; };
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, n = lane & 31, rep = a.H / a.G;
