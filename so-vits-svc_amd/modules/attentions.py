@@ -21,6 +21,12 @@ MASK_NONE, MASK_PADDING, MASK_CAUSAL = 0, 1, 2
 FUSED_TRAIN = os.environ.get("SVC_FUSED_TRAIN", "1") != "0"
 
 
+def proximal_table(T, device):
+    """The proximal bias -log1p(|i - j|) (modules/attentions.py:305-316) over the distances of T positions, as attention_scored takes it.  Made for each
+    pass and never kept: kernels read it by address, so a graph has to own the one it was captured with, and a pass's stream orders its own."""
+    return torch.arange(1 - T, T, device=device, dtype=torch.float32).abs_().log1p_().neg_()[None]
+
+
 class MultiHeadAttention(nn.Module):
     def __init__(self, channels, out_channels, n_heads, p_dropout=0., window_size=None, heads_share=True,
                  block_length=None, proximal_bias=False, proximal_init=False):
@@ -90,23 +96,19 @@ class MultiHeadAttention(nn.Module):
             return MASK_PADDING, vec
         raise NotImplementedError("attention mask is neither all-ones, causal nor an outer product of a padding mask")
 
-    def _scored_options(self, mask_mode, mask_vec, T, device):
-        """The options of svc_hip.attention_scored behind this module's: the bias -log1p(|i - j|) as a table over distances, block_length as a
+    def _scored_options(self, mask_mode, mask_vec, T, device, table=None):
+        """The options of svc_hip.attention_scored behind this module's: the bias -log1p(|i - j|) as a table over distances (`table`: the one of
+        this pass, where a stack has made it for all its layers), block_length as a
         window, the padding mask as lengths.  The padding mask must be a sequence mask (ones, then zeros: commons.sequence_mask); padded queries
         give 0 where the reference spreads them over all keys (their rows are masked behind every attention layer)."""
         opts = {"causal": mask_mode == MASK_CAUSAL, "window": self.block_length}
         if mask_mode == MASK_PADDING:
             opts["lengths"] = mask_vec.sum(1).to(torch.int32)
         if self.proximal_bias:
-            key = (T, str(device))
-            hit = self.__dict__.get("_proximal_cache")
-            if hit is None or hit[0] != key:
-                d = torch.arange(1 - T, T, device=device, dtype=torch.float32)
-                hit = self.__dict__["_proximal_cache"] = (key, (-torch.log1p(d.abs()))[None].contiguous())
-            opts["bias"] = hit[1]
+            opts["bias"] = proximal_table(T, device) if table is None else table
         return opts
 
-    def forward_train(self, x, mask_mode, mask_vec, draws=None):
+    def forward_train(self, x, mask_mode, mask_vec, draws=None, table=None):
         """Reference modules/attentions.py:198-239: separate q/k/v projections, attention as GEMMs + masked softmax, and
         `p_attn = self.drop(p_attn)` (:232) fused into the softmax kernel (`draws`: the DropoutDraws of this pass;
         without one the module draws for itself when it is in training mode with p_dropout > 0)."""
@@ -119,7 +121,7 @@ class MultiHeadAttention(nn.Module):
             if u is not None and not isinstance(u, S.HashDraw):
                 raise NotImplementedError("attention dropout from a tensor of draws with proximal_bias / block_length")
             q, k, v = (conv.forward_train(x) for conv in (self.conv_q, self.conv_k, self.conv_v))
-            att = A.attention_scored(q, k, v, self.n_heads, draw=u, p_drop=draws.p, **self._scored_options(mask_mode, mask_vec, T, x.device))
+            att = A.attention_scored(q, k, v, self.n_heads, draw=u, p_drop=draws.p, **self._scored_options(mask_mode, mask_vec, T, x.device, table))
             return self.conv_o.forward_train(att)
         if QKV_FUSED_TRAIN and self.conv_q.kernel_size == 1 and not self.conv_q.is_weight_norm and self.conv_q.bias is not None:
             # the three 1 x 1 projections as ONE 3C-row convolution whose rows are ordered (head, {q, k, v}, d): x has one consumer
@@ -139,13 +141,13 @@ class MultiHeadAttention(nn.Module):
                           mask_vec, mask_mode, drop_u=u, p_drop=draws.p)
         return self.conv_o.forward_train(att)
 
-    def forward(self, x, c, attn_mask=None, mask_mode=None, mask_vec=None):
+    def forward(self, x, c, attn_mask=None, mask_mode=None, mask_vec=None, table=None):
         if c is not x:
             raise NotImplementedError("only self-attention is used on the so-vits-svc path")
         if training_call(self.conv_q.weight) or (torch.is_grad_enabled() and x.requires_grad):
             if mask_mode is None:
                 mask_mode, mask_vec = self._mask_mode(attn_mask, x.shape[2])
-            return self.forward_train(x, mask_mode, mask_vec)
+            return self.forward_train(x, mask_mode, mask_vec, table=table)
         _no_grad_guard(self.conv_q.weight)
         B, C, T = x.shape
         if mask_mode is None:
@@ -154,7 +156,7 @@ class MultiHeadAttention(nn.Module):
         qkv = S.conv1d(x, wp, 3 * C, 1, bias=b)
         if self.scored:
             att = S.attention_scored(qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], self.n_heads,
-                                     **self._scored_options(mask_mode, mask_vec, T, x.device))
+                                     **self._scored_options(mask_mode, mask_vec, T, x.device, table))
             return self.conv_o.run(att)
         win = self.window_size or 0
         att = S.attention(qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], self.n_heads,
@@ -319,6 +321,7 @@ def _encoder_forward_train(self, x, x_mask, attn_layers, norm_a, norm_b, mask_mo
     m = x_mask[:, 0].contiguous() if x_mask.dim() == 3 else x_mask
     draws = DropoutDraws(self.p_dropout, self.training, dropout_u)
     fused = attn_layers[0].scored if len(attn_layers) else False
+    table = proximal_table(x.shape[2], x.device) if len(attn_layers) and attn_layers[0].proximal_bias else None
 
     def junction(norm, x, y):
         """norm(x + drop(y)): the dropout, the sum and the norm as one operator where no earlier form's results are to be kept."""
@@ -333,7 +336,7 @@ def _encoder_forward_train(self, x, x_mask, attn_layers, norm_a, norm_b, mask_mo
     for i in range(self.n_layers):
         if pre_layer is not None:
             x = pre_layer(i, x)
-        y = attn_layers[i].forward_train(x, mask_mode, m if mask_mode == MASK_PADDING else None, draws=draws)
+        y = attn_layers[i].forward_train(x, mask_mode, m if mask_mode == MASK_PADDING else None, draws=draws, table=table)
         x = junction(norm_a[i], x, y)
         y = self.ffn_layers[i].forward_train(x, x_mask, drop=draws)
         x = junction(norm_b[i], x, y)
@@ -396,10 +399,11 @@ class FFT(nn.Module):
         x = S.copy_bct(x, mask=m)
         H = self.hidden_channels
         gc = self.cond_layer(g) if g is not None else None
+        table = proximal_table(x.shape[2], x.device) if self.proximal_bias else None
         for i in range(self.n_layers):
             if gc is not None:      # cond_pre + conditioning + tanh*sigmoid gate: one MFMA conv with the gate epilogue
                 x = self.cond_pre.run(x, cond=gc[:, i * 2 * H:(i + 1) * 2 * H], epi=S.EPI_GATE)
-            y = self.self_attn_layers[i](x, x, mask_mode=MASK_CAUSAL)
+            y = self.self_attn_layers[i](x, x, mask_mode=MASK_CAUSAL, table=table)
             x = self.norm_layers_0[i](x, residual=y, x_mask=x_mask)
             y = self.ffn_layers[i](x, x_mask, x_is_masked=True)
             x = self.norm_layers_1[i](x, residual=y, x_mask=x_mask)

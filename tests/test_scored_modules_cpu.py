@@ -1,0 +1,35 @@
+"""What MultiHeadAttention(proximal_bias / block_length) hands to attention_scored, on the host: tables, lengths, windows and refusals (no launch)."""
+import pytest
+import torch
+
+CPU = torch.device("cpu")
+
+
+def _mha(**kw):
+    from modules.attentions import MultiHeadAttention
+    torch.manual_seed(1)
+    return MultiHeadAttention(32, 32, 2, **kw)
+
+
+def test_the_distance_table_belongs_to_its_call():
+    """A table kept by the module and replaced at another length would leave a graph that was captured with it on freed memory; one made while a
+    graph is recorded, or on another stream, would be read before it is written.  So a call's table is its own and the module holds none."""
+    from modules.attentions import MASK_NONE
+    mod = _mha(proximal_bias=True)
+    a = mod._scored_options(MASK_NONE, None, 9, CPU)["bias"]
+    b = mod._scored_options(MASK_NONE, None, 9, CPU)["bias"]
+    mod._scored_options(MASK_NONE, None, 5, CPU)
+    assert a.data_ptr() != b.data_ptr()
+    want = -torch.log1p(torch.arange(-8, 9).abs().double())[None]
+    for t in (a, b):
+        assert t.shape == (1, 17) and t.dtype == torch.float32 and (t.double() - want).abs().max() <= 2 * 2.0 ** -24 * 3      # log1p(8) < 3
+    held = [x for v in mod.__dict__.values() for x in (v if isinstance(v, tuple) else (v,)) if isinstance(x, torch.Tensor)]
+    assert not held
+
+
+def test_a_table_made_in_inference_mode_is_not_met_again_in_training():
+    from modules.attentions import MASK_NONE
+    mod = _mha(proximal_bias=True)
+    with torch.inference_mode():
+        mod._scored_options(MASK_NONE, None, 9, CPU)
+    assert not mod._scored_options(MASK_NONE, None, 9, CPU)["bias"].is_inference()      # (it could not be saved for a backward)
