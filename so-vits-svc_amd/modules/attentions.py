@@ -21,6 +21,10 @@ MASK_NONE, MASK_PADDING, MASK_CAUSAL = 0, 1, 2
 FUSED_TRAIN = os.environ.get("SVC_FUSED_TRAIN", "1") != "0"
 
 
+def _capturing(t):
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 def proximal_table(T, device):
     """The proximal bias -log1p(|i - j|) (modules/attentions.py:305-316) over the distances of T positions, as attention_scored takes it.  Made for each
     pass and never kept: kernels read it by address, so a graph has to own the one it was captured with, and a pass's stream orders its own."""
@@ -91,22 +95,36 @@ class MultiHeadAttention(nn.Module):
         vec = torch.diagonal(am[:, 0], dim1=-2, dim2=-1).contiguous().float()
         outer = vec.unsqueeze(1) * vec.unsqueeze(2)
         if bool(((am[:, 0] != 0) == (outer != 0)).all()):
-            if self.scored and bool((vec[:, 1:] > vec[:, :-1]).any()):
-                raise NotImplementedError("proximal_bias / block_length with a padding mask that is not a sequence mask (ones, then zeros)")
             return MASK_PADDING, vec
         raise NotImplementedError("attention mask is neither all-ones, causal nor an outer product of a padding mask")
 
     def _scored_options(self, mask_mode, mask_vec, T, device, table=None):
         """The options of svc_hip.attention_scored behind this module's: the bias -log1p(|i - j|) as a table over distances (`table`: the one of
         this pass, where a stack has made it for all its layers), block_length as a
-        window, the padding mask as lengths.  The padding mask must be a sequence mask (ones, then zeros: commons.sequence_mask); padded queries
+        window, the padding mask as lengths.  The padding mask must be a sequence mask (not 0, then 0: commons.sequence_mask), which costs a look from
+        the host (`_scored_attention`: while a graph is captured); padded queries
         give 0 where the reference spreads them over all keys (their rows are masked behind every attention layer)."""
         opts = {"causal": mask_mode == MASK_CAUSAL, "window": self.block_length}
         if mask_mode == MASK_PADDING:
-            opts["lengths"] = mask_vec.sum(1).to(torch.int32)
+            gone = mask_vec == 0
+            if not _capturing(mask_vec) and bool((gone[:, :-1] & ~gone[:, 1:]).any()):
+                raise NotImplementedError("proximal_bias / block_length with a padding mask that is not a sequence mask (ones, then zeros)")
+            # the first 0's place, by a binary search (a reduction over many blocks would record a memset into a captured graph)
+            opts["lengths"] = torch.searchsorted(gone.int(), torch.ones_like(gone[:, :1], dtype=torch.int32), out_int32=True)[:, 0].contiguous()
         if self.proximal_bias:
             opts["bias"] = proximal_table(T, device) if table is None else table
         return opts
+
+    def _scored_attention(self, attention, q, k, v, mask_mode, mask_vec, table, **drop):
+        """attention_scored (svc_hip's or svc_autograd's) with this module's options.  Where a captured graph keeps the host from looking at the padding
+        mask, the frames at which it is no sequence mask become NaN."""
+        T = q.shape[2]
+        opts = self._scored_options(mask_mode, mask_vec, T, q.device, table)
+        att = attention(q, k, v, self.n_heads, **drop, **opts)
+        if mask_mode == MASK_PADDING and _capturing(mask_vec):
+            other = (torch.arange(T, device=q.device) < opts["lengths"][:, None]) == (mask_vec == 0)
+            att = att.masked_fill(other[:, None], math.nan)
+        return att
 
     def forward_train(self, x, mask_mode, mask_vec, draws=None, table=None):
         """Reference modules/attentions.py:198-239: separate q/k/v projections, attention as GEMMs + masked softmax, and
@@ -121,7 +139,7 @@ class MultiHeadAttention(nn.Module):
             if u is not None and not isinstance(u, S.HashDraw):
                 raise NotImplementedError("attention dropout from a tensor of draws with proximal_bias / block_length")
             q, k, v = (conv.forward_train(x) for conv in (self.conv_q, self.conv_k, self.conv_v))
-            att = A.attention_scored(q, k, v, self.n_heads, draw=u, p_drop=draws.p, **self._scored_options(mask_mode, mask_vec, T, x.device, table))
+            att = self._scored_attention(A.attention_scored, q, k, v, mask_mode, mask_vec, table, draw=u, p_drop=draws.p)
             return self.conv_o.forward_train(att)
         if QKV_FUSED_TRAIN and self.conv_q.kernel_size == 1 and not self.conv_q.is_weight_norm and self.conv_q.bias is not None:
             # the three 1 x 1 projections as ONE 3C-row convolution whose rows are ordered (head, {q, k, v}, d): x has one consumer
@@ -155,8 +173,7 @@ class MultiHeadAttention(nn.Module):
         wp, b = self._qkv_packed()
         qkv = S.conv1d(x, wp, 3 * C, 1, bias=b)
         if self.scored:
-            att = S.attention_scored(qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], self.n_heads,
-                                     **self._scored_options(mask_mode, mask_vec, T, x.device, table))
+            att = self._scored_attention(S.attention_scored, qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], mask_mode, mask_vec, table)
             return self.conv_o.run(att)
         win = self.window_size or 0
         att = S.attention(qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], self.n_heads,

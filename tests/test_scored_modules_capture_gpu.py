@@ -61,3 +61,35 @@ def test_inference_mode_and_training_alternate(dev):
     y = fft(x.clone().requires_grad_(), m)
     y.sum().backward()
     assert (y.detach() - a).abs().max() <= 2e-4 * a.abs().max()      # (the training path's own launches: tolerance of tests/test_scored_modules_gpu.py)
+
+
+def test_padding_masks_with_holes(dev):
+    """Refused on every route; in a captured graph, where the host cannot look, the frames that a sequence mask would have otherwise are NaN."""
+    from modules.attentions import MASK_PADDING, MultiHeadAttention
+    torch.manual_seed(2)
+    mod = MultiHeadAttention(64, 64, 2, block_length=5).to(dev).eval()
+    x = torch.randn(2, 64, 60, device=dev)
+    good = (torch.arange(60, device=dev) < torch.tensor([[60], [37]], device=dev)).float()
+    bad = good.clone()
+    bad[0, 20] = 0
+    with torch.no_grad():
+        for kw in (dict(mask_mode=MASK_PADDING, mask_vec=bad), dict(attn_mask=(bad[:, None, :, None] * bad[:, None, None]))):
+            with pytest.raises(NotImplementedError, match="sequence mask"):
+                mod(x, x, **kw)
+        with pytest.raises(NotImplementedError, match="sequence mask"):
+            mod.forward_train(x, MASK_PADDING, bad)
+        want = mod(x, x, mask_mode=MASK_PADDING, mask_vec=good).clone()
+        assert torch.equal(mod(x, x, attn_mask=good[:, None, :, None] * good[:, None, None]), want)
+        held = good.clone()
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = mod(x, x, mask_mode=MASK_PADDING, mask_vec=held)
+        for m in (good, bad, good, bad):
+            held.copy_(m)
+            gr.replay()
+            torch.cuda.synchronize()
+            if m is good:
+                assert torch.equal(out, want)
+            else:           # first 0 at 20 by the search or 60: the frames that differ from the mask are marked, and no other item's
+                assert torch.isnan(out[0]).any() and torch.equal(out[1], want[1])

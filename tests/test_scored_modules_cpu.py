@@ -33,3 +33,21 @@ def test_a_table_made_in_inference_mode_is_not_met_again_in_training():
     with torch.inference_mode():
         mod._scored_options(MASK_NONE, None, 9, CPU)
     assert not mod._scored_options(MASK_NONE, None, 9, CPU)["bias"].is_inference()      # (it could not be saved for a backward)
+
+
+@pytest.mark.parametrize("mask", [[[1, 1, 0, 1, 0]], [[0, 1, 1, 1, 1]], [[1, 1, 1, 1, 1], [1, 0, 1, 1, 0]], [[0, 0, 0, 0, 1]]])
+def test_a_padding_mask_with_a_hole_is_refused_whatever_the_route(mask):
+    """mask_mode=MASK_PADDING with a mask that is not ones, then zeros: its sum is not a length."""
+    from modules.attentions import MASK_PADDING
+    for mod in (_mha(proximal_bias=True), _mha(block_length=2)):
+        with pytest.raises(NotImplementedError, match="sequence mask"):
+            mod._scored_options(MASK_PADDING, torch.tensor(mask, dtype=torch.float32), 5, CPU)
+
+
+@pytest.mark.parametrize("mask,want", [([[1, 1, 0, 0, 0], [1, 1, 1, 1, 1], [0, 0, 0, 0, 0]], [2, 5, 0]), ([[0.25, 3.0, 2.0, 0, 0]], [3]), ([[1.0]], [1]), ([[0.0]], [0])])
+def test_lengths_count_the_places_that_are_not_zero(mask, want):
+    """A place belongs to the item where the mask is not 0 (masked_fill(mask == 0)), whatever its value."""
+    from modules.attentions import MASK_PADDING
+    mod = _mha(block_length=2)
+    got = mod._scored_options(MASK_PADDING, torch.tensor(mask, dtype=torch.float32), len(mask[0]), CPU)["lengths"]
+    assert got.dtype == torch.int32 and got.tolist() == want and got.is_contiguous()
