@@ -98,13 +98,13 @@ class MultiHeadAttention(nn.Module):
             return MASK_PADDING, vec
         raise NotImplementedError("attention mask is neither all-ones, causal nor an outer product of a padding mask")
 
-    def _scored_options(self, mask_mode, mask_vec, T, device, table=None):
+    def _scored_options(self, mask_mode, mask_vec, T, device, table=None, masked=True):
         """The options of svc_hip.attention_scored behind this module's: the bias -log1p(|i - j|) as a table over distances (`table`: the one of
         this pass, where a stack has made it for all its layers), block_length as a
-        window, the padding mask as lengths.  The padding mask must be a sequence mask (not 0, then 0: commons.sequence_mask), which costs a look from
+        window where the call has a mask (:223-229), the padding mask as lengths.  The padding mask must be a sequence mask (not 0, then 0: commons.sequence_mask), which costs a look from
         the host (`_scored_attention`: while a graph is captured); padded queries
         give 0 where the reference spreads them over all keys (their rows are masked behind every attention layer)."""
-        opts = {"causal": mask_mode == MASK_CAUSAL, "window": self.block_length}
+        opts = {"causal": mask_mode == MASK_CAUSAL, "window": self.block_length if masked else None}
         if mask_mode == MASK_PADDING:
             gone = mask_vec == 0
             if not _capturing(mask_vec) and bool((gone[:, :-1] & ~gone[:, 1:]).any()):
@@ -115,21 +115,21 @@ class MultiHeadAttention(nn.Module):
             opts["bias"] = proximal_table(T, device) if table is None else table
         return opts
 
-    def _scored_attention(self, attention, q, k, v, mask_mode, mask_vec, table, **drop):
+    def _scored_attention(self, attention, q, k, v, mask_mode, mask_vec, table, masked=True, **drop):
         """attention_scored (svc_hip's or svc_autograd's) with this module's options.  Where a captured graph keeps the host from looking at the padding
         mask, the frames at which it is no sequence mask become NaN."""
         T = q.shape[2]
-        opts = self._scored_options(mask_mode, mask_vec, T, q.device, table)
+        opts = self._scored_options(mask_mode, mask_vec, T, q.device, table, masked)
         att = attention(q, k, v, self.n_heads, **drop, **opts)
         if mask_mode == MASK_PADDING and _capturing(mask_vec):
             other = (torch.arange(T, device=q.device) < opts["lengths"][:, None]) == (mask_vec == 0)
             att = att.masked_fill(other[:, None], math.nan)
         return att
 
-    def forward_train(self, x, mask_mode, mask_vec, draws=None, table=None):
+    def forward_train(self, x, mask_mode, mask_vec, draws=None, table=None, masked=True):
         """Reference modules/attentions.py:198-239: separate q/k/v projections, attention as GEMMs + masked softmax, and
         `p_attn = self.drop(p_attn)` (:232) fused into the softmax kernel (`draws`: the DropoutDraws of this pass;
-        without one the module draws for itself when it is in training mode with p_dropout > 0)."""
+        without one the module draws for itself when it is in training mode with p_dropout > 0).  `masked`: the call has a mask, if one of all ones."""
         win = self.window_size or 0
         if draws is None:
             draws = DropoutDraws(self.p_dropout, self.training)
@@ -139,7 +139,7 @@ class MultiHeadAttention(nn.Module):
             if u is not None and not isinstance(u, S.HashDraw):
                 raise NotImplementedError("attention dropout from a tensor of draws with proximal_bias / block_length")
             q, k, v = (conv.forward_train(x) for conv in (self.conv_q, self.conv_k, self.conv_v))
-            att = self._scored_attention(A.attention_scored, q, k, v, mask_mode, mask_vec, table, draw=u, p_drop=draws.p)
+            att = self._scored_attention(A.attention_scored, q, k, v, mask_mode, mask_vec, table, masked, draw=u, p_drop=draws.p)
             return self.conv_o.forward_train(att)
         if QKV_FUSED_TRAIN and self.conv_q.kernel_size == 1 and not self.conv_q.is_weight_norm and self.conv_q.bias is not None:
             # the three 1 x 1 projections as ONE 3C-row convolution whose rows are ordered (head, {q, k, v}, d): x has one consumer
@@ -162,10 +162,11 @@ class MultiHeadAttention(nn.Module):
     def forward(self, x, c, attn_mask=None, mask_mode=None, mask_vec=None, table=None):
         if c is not x:
             raise NotImplementedError("only self-attention is used on the so-vits-svc path")
+        masked = attn_mask is not None or mask_mode is not None
         if training_call(self.conv_q.weight) or (torch.is_grad_enabled() and x.requires_grad):
             if mask_mode is None:
                 mask_mode, mask_vec = self._mask_mode(attn_mask, x.shape[2])
-            return self.forward_train(x, mask_mode, mask_vec, table=table)
+            return self.forward_train(x, mask_mode, mask_vec, table=table, masked=masked)
         _no_grad_guard(self.conv_q.weight)
         B, C, T = x.shape
         if mask_mode is None:
@@ -173,7 +174,7 @@ class MultiHeadAttention(nn.Module):
         wp, b = self._qkv_packed()
         qkv = S.conv1d(x, wp, 3 * C, 1, bias=b)
         if self.scored:
-            att = self._scored_attention(S.attention_scored, qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], mask_mode, mask_vec, table)
+            att = self._scored_attention(S.attention_scored, qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], mask_mode, mask_vec, table, masked)
             return self.conv_o.run(att)
         win = self.window_size or 0
         att = S.attention(qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], self.n_heads,

@@ -93,3 +93,17 @@ def test_padding_masks_with_holes(dev):
                 assert torch.equal(out, want)
             else:           # first 0 at 20 by the search or 60: the frames that differ from the mask are marked, and no other item's
                 assert torch.isnan(out[0]).any() and torch.equal(out[1], want[1])
+
+
+def test_block_length_without_a_mask_cuts_nothing(dev):
+    """(modules/attentions.py:223-229: the block is inside the mask's branch)"""
+    from modules.attentions import MASK_NONE, MultiHeadAttention
+    torch.manual_seed(4)
+    mod, wide = (MultiHeadAttention(64, 64, 2, block_length=n).to(dev).eval() for n in (3, 100))
+    wide.load_state_dict(mod.state_dict())
+    x = torch.randn(2, 64, 50, device=dev)
+    with torch.no_grad():
+        everything = wide(x, x, mask_mode=MASK_NONE)
+        assert torch.equal(mod(x, x), everything)
+        cut = mod(x, x, attn_mask=torch.ones(1, 1, 50, 50, device=dev))
+        assert torch.equal(cut, mod(x, x, mask_mode=MASK_NONE)) and not torch.equal(cut, everything)

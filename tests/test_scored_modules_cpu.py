@@ -51,3 +51,28 @@ def test_lengths_count_the_places_that_are_not_zero(mask, want):
     mod = _mha(block_length=2)
     got = mod._scored_options(MASK_PADDING, torch.tensor(mask, dtype=torch.float32), len(mask[0]), CPU)["lengths"]
     assert got.dtype == torch.int32 and got.tolist() == want and got.is_contiguous()
+
+
+def test_block_length_goes_with_a_mask(monkeypatch):
+    """modules/attentions.py:223-229: the block is cut out of the scores where a mask is given, not without one."""
+    import modules.attentions as M
+    mod = _mha(block_length=2).eval()
+    seen = []
+    monkeypatch.setattr(M.S, "conv1d", lambda x, *a, **kw: torch.zeros(x.shape[0], 96, x.shape[2]))
+    monkeypatch.setattr(mod, "_qkv_packed", lambda: (None, None))
+    monkeypatch.setattr(type(mod.conv_o), "run", lambda self, x: x)
+    monkeypatch.setattr(M.S, "attention_scored", lambda q, k, v, n, **kw: seen.append(kw["window"]) or q)
+    x = torch.zeros(1, 32, 6)
+    with torch.no_grad():
+        mod(x, x)
+        mod(x, x, attn_mask=torch.ones(1, 1, 6, 6))
+        mod(x, x, mask_mode=M.MASK_CAUSAL)
+        mod(x, x, mask_mode=M.MASK_NONE)              # a caller's promise that its mask is all ones
+    assert seen == [None, 2, 2, 2]
+    seen.clear()
+    monkeypatch.setattr(type(mod.conv_o), "forward_train", lambda self, x, **kw: x)
+    monkeypatch.setattr(M.A, "attention_scored", lambda q, k, v, n, **kw: seen.append(kw["window"]) or q)
+    y = x.requires_grad_()
+    mod(y, y)
+    mod(y, y, attn_mask=torch.ones(1, 1, 6, 6))
+    assert seen == [None, 2]
