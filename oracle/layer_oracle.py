@@ -52,6 +52,32 @@ def visible(B, Tq, Tk, causal=False, window=None, prefix=None, docs=None, length
     return see, pos
 
 
+def visible_matrix(B, Tq, Tk, causal=False, window=None, prefix=None, docs=None, lengths=None, offset=None):
+    """visible() by comparisons of whole matrices, for long sequences."""
+    see, pos, s = torch.zeros(B, Tq, Tk, dtype=torch.bool), torch.zeros(B, Tq, dtype=torch.long), torch.arange(Tk)
+    for b in range(B):
+        off = Tk - Tq if offset is None else int(offset[b]) if isinstance(offset, torch.Tensor) else offset
+        n = Tk if lengths is None else min(max(int(lengths[b]), 0), Tk)
+        p = pos[b] = off + torch.arange(Tq)
+        start, front = torch.zeros(Tq, dtype=torch.long), torch.full((Tq,), 0 if prefix is None or docs is not None else int(prefix[b]))
+        ok = ((p >= 0) & (p < n))[:, None] & (s < n)
+        if docs is not None:
+            mine = torch.zeros_like(ok)
+            for i, (lo, hi) in enumerate(zip(docs[b].tolist(), docs[b].tolist()[1:])):
+                own = (lo <= p) & (p < hi)
+                mine |= own[:, None] & (lo <= s) & (s < hi)
+                start[own] = lo
+                if prefix is not None:
+                    front[own] = int(prefix[b, i])
+            ok &= mine
+        if causal:
+            ok &= (s <= p[:, None]) | (s < (start + front)[:, None])
+        if window is not None:
+            ok &= (s - p[:, None]).abs() <= window
+        see[b] = ok
+    return see, pos
+
+
 def attention(q, k, v, n_heads, dout=None, bias=None, softcap=0.0, scale=None, draw=None, p_drop=0.0, **mask):
     """-> dict of out (dq, dk, dv, dbias) and, under "mag_<name>", the sums of absolute values behind them; "score": the largest sum of |q||k| scale."""
     q, k, v = (x.detach().cpu().double() for x in (q, k, v))
