@@ -165,6 +165,13 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
           const int2 w = ivs[cur][32 * rt + pos_of(i, h)];
           x[i] = s >= w.x && s < w.y ? x[i] : 0.f;
         }
+        if (sc.cap) {                                        // (what lies at keys that no query sees may be nan, and so its cap factor, by which 0 is multiplied below)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int2 w = ivs[cur][32 * rt + pos_of(i, h)];
+            th[i] = s >= w.x && s < w.y ? th[i] : 0.f;
+          }
+        }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] = x[i];

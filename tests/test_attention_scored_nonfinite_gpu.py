@@ -1,0 +1,46 @@
+"""attention_scored where values are not finite or very large: what a query sees decides what it answers, in every kernel alike."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+NAN, INF = float("nan"), float("inf")
+
+
+def _inputs(dev, dt, B, H, G, dk, Tq, Tk, seed=0):
+    g = torch.Generator().manual_seed(seed + Tq + 7 * Tk + dk)
+    return [torch.randn(B, n * dk, T, generator=g).to(dt).to(dev) for n, T in ((H, Tq), (G, Tk), (G, Tk), (H, Tq))]
+
+
+def _pass(q, k, v, do, H, **kw):
+    """(out, lse, dq, dk, dv, dbias or None) of a training pass."""
+    import svc_hip as S
+    out, lse, o32 = S.attention_scored_fwd(q, k, v, H, want_dbias="bias" in kw, **kw)
+    return (out, lse, *S.attention_scored_bwd(do, q, k, v, out if o32 is None else o32, lse, H, want_dbias="bias" in kw, **kw))
+
+
+@pytest.mark.parametrize("p", [0.0, 0.2])
+@pytest.mark.parametrize("table", [False, True])
+@pytest.mark.parametrize("dk", [64, 96, 128])
+@pytest.mark.parametrize("dt", TYPES)
+def test_capped_scores_at_keys_that_no_query_sees(dev, dt, dk, table, p):
+    """Keys behind the last query's position, and before the first one's window, inside the key blocks of keys that are seen: with a cap the factor
+    1 - tanh^2 of a NaN score is NaN, whatever its P."""
+    import svc_hip as S
+    q, k, v, do = _inputs(dev, TYPES[dt], 2, 2, 1, dk, 75, 150)
+    kw = dict(softcap=4.0, offset=41)
+    if table:
+        kw["bias"] = torch.linspace(-1, 1, 2 * 11, device=dev).view(2, 11)
+    if p:
+        kw.update(draw=S.HashDraw(torch.tensor([3], device=dev), 1), p_drop=p)
+    for seen, more in ((slice(0, 116), dict(causal=True)), (slice(36, 121), dict(window=5))):
+        want = _pass(q, k, v, do, 2, **kw, **more)
+        for bad in (NAN, INF):
+            k2, v2 = torch.full_like(k, bad), torch.full_like(v, bad)
+            k2[:, :, seen], v2[:, :, seen] = k[:, :, seen], v[:, :, seen]
+            for a, b in zip(want, _pass(q, k2, v2, do, 2, **kw, **more)):
+                assert a is None or torch.equal(a, b)
+        for g in want[3:5]:
+            g = g.clone()
+            g[:, :, seen] = 0
+            assert not g.any()
