@@ -180,7 +180,8 @@ __global__ __launch_bounds__(256, DP > (sizeof(E) == 4 ? 64 : 96) ? 1 : 2) void 
 #pragma unroll
   for (int w = 0; w < 4; ++w) mc = fmaxf(mc, ms(w)[c]);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) lsum += ms(w)[c] == -INFINITY ? 0.f : ls(w)[c] * __builtin_amdgcn_exp2f(ms(w)[c] - mc);
+  for (int w = 0; w < 4; ++w)          // (a wave without a maximum has the sum 0, or nan where its scores are)
+    lsum = fmaf(ls(w)[c], ms(w)[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms(w)[c] - mc), lsum);
   const float* const f = (const float*)lds_ + c;
   constexpr int FW = WAVE / 4;
   if (sp.parts > 1) {
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(256, DP > (sizeof(E) == 4 ? 64 : 96) ? 1 : 2) void 
     float inv = lsum > 0.f ? 1.f / lsum : 0.f;
     if (lsum != lsum) inv = lsum;
     if (a.seed) inv *= 65536.f / (65536.f - (float)thr);
-    if (a.lse && tid < 32) a.lse[row] = lsum > 0.f ? mc - PUP<E> + __builtin_amdgcn_logf(lsum) : 0.f;
+    if (a.lse && tid < 32) a.lse[row] = lsum > 0.f || lsum != lsum ? mc - PUP<E> + __builtin_amdgcn_logf(lsum) : 0.f;
     E* y = (E*)a.out + b * a.o_bs + (long long)hc * a.dk * a.o_cs + tc;
     float* y32 = a.out32 ? a.out32 + ((long long)b * a.H + hc) * a.dk * a.Tq + tc : nullptr;
     for (int d = tid >> 5; d < a.dk; d += 8) {
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(256) void join_kernel(svc_attn_scored_t a, Split sp
   if (l != l) inv = l;
   if (a.seed) inv *= 65536.f / (65536.f - rintf(a.p_drop * 65536.f));
   const int head = kvh * (a.H / a.G) + c / a.Tq, t = c % a.Tq;
-  if (a.lse && d == 0) a.lse[((long long)b * a.H + head) * a.Tq + t] = l > 0.f ? m - PUP<E> + __builtin_amdgcn_logf(l) : 0.f;
+  if (a.lse && d == 0) a.lse[((long long)b * a.H + head) * a.Tq + t] = l > 0.f || l != l ? m - PUP<E> + __builtin_amdgcn_logf(l) : 0.f;
   v *= inv;
   ((E*)a.out)[b * a.o_bs + ((long long)head * a.dk + d) * a.o_cs + t] = (E)v;
   if (a.out32) a.out32[(((long long)b * a.H + head) * a.dk + d) * a.Tq + t] = v;

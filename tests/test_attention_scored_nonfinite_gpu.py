@@ -44,3 +44,31 @@ def test_capped_scores_at_keys_that_no_query_sees(dev, dt, dk, table, p):
             g = g.clone()
             g[:, :, seen] = 0
             assert not g.any()
+
+
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("T", [40, 64, 65, 150])
+@pytest.mark.parametrize("dk", [32, 96, 128])
+@pytest.mark.parametrize("dt", TYPES)
+def test_a_nan_query_spoils_its_row_alone(dev, dt, dk, T, cap):
+    """Up to 64 queries and beyond (two forward kernels): out, lse and dq are NaN at the query, dv at the keys that it sees, nothing else is."""
+    q, k, v, do = _inputs(dev, TYPES[dt], 1, 2, 1, dk, T, T)
+    t0, w = 21, 5
+    q[0, 3, t0] = NAN                                                  # head 0
+    out, lse, dq, _, dv, _ = _pass(q, k, v, do, 2, window=w, softcap=cap)
+    rows = torch.zeros(1, 2, T, dtype=torch.bool, device=dev)
+    rows[0, 0, t0] = True
+    wide = rows[:, :, None].expand(1, 2, dk, T).reshape(1, 2 * dk, T)
+    keys = ((torch.arange(T, device=dev) - t0).abs() <= w).expand(1, dk, T)
+    assert torch.equal(torch.isnan(lse), rows)
+    for x, where in ((out, wide), (dq, wide), (dv, keys)):
+        assert torch.equal(torch.isnan(x), where) and not torch.isinf(x).any()
+
+
+@pytest.mark.parametrize("T", [1, 40, 150])
+@pytest.mark.parametrize("dt", TYPES)
+def test_a_row_whose_every_score_is_nan_has_a_nan_lse(dev, dt, T):
+    q, k, v, do = _inputs(dev, TYPES[dt], 1, 1, 1, 64, T, 700)
+    q[0, 0] = NAN
+    for x in _pass(q, k, v, do, 1)[:3]:
+        assert torch.isnan(x).all()
