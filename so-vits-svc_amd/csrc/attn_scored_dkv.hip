@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float g = fmaf(p[i], dp[i], -(x[i] * rows[cur][32 * rt + pos_of(i, h)]));
-          x[i] = whole || x[i] > 0.f ? g : 0.f;
+          x[i] = whole || x[i] != 0.f ? g : 0.f;             // (a nan P is not a masked one)
         }
       } else {
         if (DROP && (EARLY || a.seed)) {
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float g = x[i] * (dp[i] - rows[cur][32 * rt + pos_of(i, h)]);
-          x[i] = whole || x[i] > 0.f ? g : 0.f;              // (a masked entry: 0 whatever dO.v is)
+          x[i] = whole || x[i] != 0.f ? g : 0.f;             // (a masked entry: 0 whatever dO.v is; a nan P is not one)
         }
       }
       if (sc.cap) {

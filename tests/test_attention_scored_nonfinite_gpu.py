@@ -65,6 +65,23 @@ def test_a_nan_query_spoils_its_row_alone(dev, dt, dk, T, cap):
         assert torch.equal(torch.isnan(x), where) and not torch.isinf(x).any()
 
 
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("T", [60, 150])
+@pytest.mark.parametrize("dk", [32, 96, 128])
+@pytest.mark.parametrize("dt", TYPES)
+def test_a_nan_key_spoils_the_rows_that_see_it(dev, dt, dk, T, cap):
+    """Rows that see it are NaN, and so are dk and dv of every key that one of these rows sees: P of such a row is NaN at all of them."""
+    q, k, v, do = _inputs(dev, TYPES[dt], 1, 2, 1, dk, T, T)
+    s0, w = 30, 4
+    k[0, 1, s0] = NAN
+    out, lse, _, dk_, dv, _ = _pass(q, k, v, do, 2, window=w, softcap=cap)
+    at = (torch.arange(T, device=dev) - s0).abs()
+    assert torch.equal(torch.isnan(lse), (at <= w).expand(1, 2, T))
+    assert torch.equal(torch.isnan(out), (at <= w).expand(1, 2 * dk, T))
+    for x in (dk_, dv):
+        assert torch.equal(torch.isnan(x), (at <= 2 * w).expand(1, dk, T))
+
+
 @pytest.mark.parametrize("T", [1, 40, 150])
 @pytest.mark.parametrize("dt", TYPES)
 def test_a_row_whose_every_score_is_nan_has_a_nan_lse(dev, dt, T):
