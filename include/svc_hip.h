@@ -757,6 +757,8 @@ int svc_cmag_bwd_f32(const float* re, const float* im, const float* mag, const f
  * bias: fp32 [bias_heads][2 bias_w + 1] contiguous, bias_heads = H or 1; its gradient dbias has the same shape (NULL: not wanted).  An entry of -65504
  * (fp16's lowest value) or below masks its distance.
  * Accumulation, softmax statistics and gradients of the bias are fp32 for every dtype; P and dS are rounded to dtype as operands.
+ * Not finite: a NaN score makes its query's out and lse NaN, and with them dk and dv of the keys that the query sees.  An infinite score of minus sign is a key
+ * without weight; infinite v that are seen give infinities of their sign (a 16-bit type's pass with out32, whose P has several operands: infinities or NaN).
  *
  * svc_attn_scored_fwd writes out and, when not NULL, lse [B,H,Tq] (log2 of the sum of exp2 of the scores in log2 units; 0 for a query
  * without keys) and out32 [B,H*dk,Tq], contiguous: the output in fp32, from which 16-bit types' backward takes its row sums of dO out.

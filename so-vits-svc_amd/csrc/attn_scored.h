@@ -51,14 +51,36 @@ __device__ __forceinline__ void rest2(float& x, float& y, unsigned u) {
   x -= __builtin_bit_cast(float, u << 16);
   y -= __builtin_bit_cast(float, u & 0xffff0000u);
 }
-__device__ __forceinline__ void split3(float x, float y, unsigned& a, unsigned& b, unsigned& c) {
+// Two values' parts; `big` collects the largest magnitude.  Where that passes bf16's own (an infinity, or a number that rounds to one) the caller has the parts
+// made by split3_large: a test a tile, where a test a value took two instructions of ten.  (nan: all three parts are nan.)
+constexpr float BF16_TOP = 0x1.fep127f;
+__device__ __forceinline__ void split3(float x, float y, unsigned& a, unsigned& b, unsigned& c, float& big) {
+  big = fmaxf(fmaxf(fabsf(x), fabsf(y)), big);
   a = pack2(x, y);
   rest2(x, y, a);
-  x = fabsf(x) < INFINITY ? x : 0.f;      // (an infinity or nan is its first part alone)
-  y = fabsf(y) < INFINITY ? y : 0.f;
   b = pack2(x, y);
   rest2(x, y, b);
   c = pack2(x, y);
+}
+// An infinity is 1, 0 and, as its third part, itself with its sign: of the six products only the one with the other operand's first part meets it, so an
+// infinite operand gives an infinity of the right sign (as a first part it would meet the other's smaller parts, which are of either sign or 0: nan).  A number that
+// would round to infinity is cut to its first part instead.
+__device__ __forceinline__ void split3_large(float x, float y, unsigned& a, unsigned& b, unsigned& c) {
+  a = pack2(x, y);
+  unsigned top[2], third[2];
+  float v[2] = {x, y};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const unsigned u = __builtin_bit_cast(unsigned, v[i]);
+    const bool inf = (u & 0x7fffffffu) == 0x7f800000u;
+    top[i] = inf ? (u >> 16 & 0x8000u) | 0x3f80u : fabsf(v[i]) > BF16_TOP ? u >> 16 : a >> 16 * i & 0xffffu;
+    third[i] = inf ? u >> 16 : 0u;
+    v[i] = inf ? 0.f : v[i] - __builtin_bit_cast(float, top[i] << 16);
+  }
+  a = top[0] | top[1] << 16;
+  b = pack2(v[0], v[1]);
+  rest2(v[0], v[1], b);
+  c = pack2(v[0], v[1]) | third[0] | third[1] << 16;
 }
 
 // A staged tile: rows of RB bytes of positions.  128-byte rows (64 positions of a 16-bit type, 32 of fp32); 64-byte rows for the backward at 128
@@ -259,16 +281,30 @@ struct Source {                         // one head's matrix as this thread sees
     }
     if constexpr (X3<E>) {
       static_assert(RB == 128, "32 positions");
-#pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const f32x4 x = __builtin_bit_cast(f32x4, f.v[i]);
-        uint2 u, v, w;
-        split3(x[0], x[1], u.x, v.x, w.x);
-        split3(x[2], x[3], u.y, v.y, w.y);
+      float big = 0.f;
+      auto put = [&](int i, uint2 u, uint2 v, uint2 w) {
         char* o = (char*)lds + (tid / CH + i * RS) * X3_PITCH + (tid & (CH - 1)) * 8;
         *(uint2*)o = u;
         *(uint2*)(o + DP * X3_PITCH) = v;
         *(uint2*)(o + 2 * DP * X3_PITCH) = w;
+      };
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        const f32x4 x = __builtin_bit_cast(f32x4, f.v[i]);
+        uint2 u, v, w;
+        split3(x[0], x[1], u.x, v.x, w.x, big);
+        split3(x[2], x[3], u.y, v.y, w.y, big);
+        put(i, u, v, w);
+      }
+      if (__any(big > BF16_TOP)) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          const f32x4 x = __builtin_bit_cast(f32x4, f.v[i]);
+          uint2 u, v, w;
+          split3_large(x[0], x[1], u.x, v.x, w.x);
+          split3_large(x[2], x[3], u.y, v.y, w.y);
+          put(i, u, v, w);
+        }
       }
       return;
     }
@@ -392,8 +428,13 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
   if constexpr (X3<E>) {
     const char* q = (const char*)lds + (lane & 31) * X3_PITCH + 2 * (32 * rt + 8 * h);
     union { unsigned u[4]; bf16x8 v; } b[2][3];
+    float big = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) split3(w[2 * e], w[2 * e + 1], b[e >> 2][0].u[e & 3], b[e >> 2][1].u[e & 3], b[e >> 2][2].u[e & 3]);
+    for (int e = 0; e < 8; ++e) split3(w[2 * e], w[2 * e + 1], b[e >> 2][0].u[e & 3], b[e >> 2][1].u[e & 3], b[e >> 2][2].u[e & 3], big);
+    if (__any(big > BF16_TOP)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) split3_large(w[2 * e], w[2 * e + 1], b[e >> 2][0].u[e & 3], b[e >> 2][1].u[e & 3], b[e >> 2][2].u[e & 3]);
+    }
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) {
       f32x16 small;

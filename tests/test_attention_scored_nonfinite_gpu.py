@@ -89,3 +89,83 @@ def test_a_row_whose_every_score_is_nan_has_a_nan_lse(dev, dt, T):
     q[0, 0] = NAN
     for x in _pass(q, k, v, do, 1)[:3]:
         assert torch.isnan(x).all()
+
+
+def _exact(q, k, v, H, see):
+    """float64, over the seen keys alone: a masked key takes no part, whatever it holds."""
+    B, C, Tq = q.shape
+    dk = C // H
+    G = k.shape[1] // dk
+    q, k, v = (x.double().cpu() for x in (q, k, v))
+    out = torch.zeros_like(q)
+    for b in range(B):
+        for h in range(H):
+            Q, K, V = q[b, h * dk:(h + 1) * dk], k[b, h // (H // G) * dk:][:dk], v[b, h // (H // G) * dk:][:dk]
+            for t in range(Tq):
+                s = torch.nonzero(see[t])[:, 0]
+                a = (Q[:, t, None] * K[:, s]).sum(0) * dk ** -0.5
+                P = torch.exp(a - a.max())
+                live = P > 0
+                out[b, h * dk:(h + 1) * dk, t] = (V[:, s[live]] * P[live]).sum(1) / P.sum()
+    return out
+
+
+@pytest.mark.parametrize("dk", [20, 64, 96, 128])
+@pytest.mark.parametrize("T", [30, 150])
+@pytest.mark.parametrize("dt", TYPES)
+def test_infinite_values(dev, dt, T, dk):
+    """An infinity that is seen gives infinities of its sign, not NaN: fp32's products of three parts as well."""
+    import svc_hip as S
+    q, k, v, _ = _inputs(dev, TYPES[dt], 1, 2, 1, dk, T, T)
+    v[0, 0, 17], v[0, 5, 3], v[0, 6, T - 1] = INF, -INF, INF
+    v[0, 7] = 1.0                                                      # a part of 1.0 behind the first is 0
+    v[0, 7, 4] = -INF
+    want = _exact(q, k, v, 2, torch.ones(T, T, dtype=torch.bool))
+    got = S.attention_scored(q, k, v, 2).double().cpu()
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and not torch.isnan(got).any()
+    hot = torch.isinf(want)
+    assert torch.equal(got[hot], want[hot])
+    u = max(torch.finfo(TYPES[dt]).eps / 2, 2.0 ** -24 * 8 * dk)
+    # u for the result, u for P as an operand, of sums of |v| P with |v| < 6
+    assert (got - want)[~hot].abs().max() <= 2 * u * 6
+    # a training pass of a 16-bit type has P in several operands, whose rests are of either sign or 0: not finite at the same places, and the same elsewhere
+    train = S.attention_scored_fwd(q, k, v, 2)[0].double().cpu()
+    assert torch.equal(~torch.isfinite(train), hot) and (train - want)[~hot].abs().max() <= 2 * u * 6
+    assert dt != "fp32" or torch.equal(train, got)
+
+
+@pytest.mark.parametrize("T", [30, 150])
+@pytest.mark.parametrize("dt", TYPES)
+def test_infinite_keys(dev, dt, T):
+    """A score of minus infinity is a key without weight: the other keys' rows, and dk and dv, are as if it were not there."""
+    import svc_hip as S
+    dt = TYPES[dt]
+    q, k, v, do = _inputs(dev, dt, 1, 2, 1, 64, T, T)
+    q[0, 2], q[0, 64 + 2] = q[0, 2].abs() + 0.5, q[0, 64 + 2].abs() + 0.5
+    k[0, 2, 11] = -INF
+    see = torch.ones(T, T, dtype=torch.bool)
+    see[:, 11] = False
+    want = _exact(q, k, v, 2, see)
+    out, lse, dq, dk_, dv, _ = _pass(q, k, v, do, 2)
+    u = max(torch.finfo(dt).eps / 2, 2.0 ** -24 * 8 * 64)
+    for got in (out, S.attention_scored(q, k, v, 2)):
+        assert (got.double().cpu() - want).abs().max() <= 2 * u * 6
+    assert torch.isfinite(lse).all() and torch.isfinite(dk_).all() and torch.isfinite(dv).all()
+    assert not dk_[0, :, 11].any() and not dv[0, :, 11].any()
+    dq = dq.view(1, 2, 64, T)
+    assert torch.isfinite(dq[:, :, :2]).all() and torch.isfinite(dq[:, :, 3:]).all()      # (channel 2: 0 * infinity)
+
+
+def test_the_largest_fp32_values(dev):
+    """A row of one key answers with its v, up to where the type ends: 3.399e38 rounds to infinity in bf16.  (P is 2 to the rounding of the maximum, some half
+    steps from 1, and divided by itself; at the type's very last number a P of 1 + 2^-23 would overflow.)"""
+    import svc_hip as S
+    top = 3.399e38
+    q, k, v, _ = _inputs(dev, torch.float32, 2, 2, 1, 48, 100, 100)
+    v[0, :, 0], v[1, :, 0] = top, -top
+    v[0, 3, 0], v[1, 4, 0] = 3.3e38, 2.0 ** 127
+    n = torch.tensor([1, 1], dtype=torch.int32, device=dev)
+    out = S.attention_scored(q, k, v, 2, lengths=n)
+    for h in (out[:, :48, 0], out[:, 48:, 0]):
+        assert ((h.double() - v[:, :, 0].double()).abs() <= 8 * 2.0 ** -24 * v[:, :, 0].double().abs()).all()
+    assert not out[:, :, 1:].any()
