@@ -2062,9 +2062,6 @@ def _drop_args(what, a, draw, p, dev):
     return False
 
 
-SIDE_FIELDS = {"prefix": "prefix", "docs": "docs", "lengths": "lengths", "offset": "offsets"}      # a call's int32 side tensors and their fields
-
-
 def _attn_scored_args(q, k, v, n_heads, bias, softcap, scale, causal, window, prefix, docs, lengths, offset, draw, p_drop):
     what = "attention_scored"
     dev, code = _typed(what, q, k, v)

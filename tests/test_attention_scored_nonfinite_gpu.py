@@ -169,3 +169,37 @@ def test_the_largest_fp32_values(dev):
     for h in (out[:, :48, 0], out[:, 48:, 0]):
         assert ((h.double() - v[:, :, 0].double()).abs() <= 8 * 2.0 ** -24 * v[:, :, 0].double().abs()).all()
     assert not out[:, :, 1:].any()
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_saved_tensors_that_come_back_at_the_same_address_with_other_strides(dev, dt):
+    """Hooks that move saved tensors away and back may be given the old memory again: the backward has to look at the strides, not at the address alone."""
+    import svc_autograd as A
+    B, C, T = 2, 64, 40
+    dt = TYPES[dt]
+    g = torch.Generator().manual_seed(1)
+    hold = torch.randn(B, 2 * C, T, generator=g).to(dt).to(dev)              # q: the first half of the channels
+    k, v, do = (torch.randn(B, C, T, generator=g).to(dt).to(dev) for _ in range(3))
+    go = lambda q: (A.attention_scored(q, k, v, 2, causal=True), q)  # noqa: E731
+    k.requires_grad_(), v.requires_grad_()
+    y, q = go(hold[:, :C].clone().requires_grad_())
+    want = torch.autograd.grad(y, (q, k, v), do)
+    q = hold[:, :C].detach().requires_grad_()
+
+    def pack(t):
+        return (t.detach().clone(), True) if t.data_ptr() == q.data_ptr() else (t, False)
+
+    def unpack(pair):
+        t, moved = pair
+        if not moved:
+            return t
+        back = hold.view(-1)[:B * C * T].view(B, C, T)                       # at its old address, contiguous
+        back.copy_(t)
+        hold[1] = 7.0                                                        # (the rest of the old memory is someone else's by now)
+        return back
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        y, _ = go(q)
+    got = torch.autograd.grad(y, (q, k, v), do)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)

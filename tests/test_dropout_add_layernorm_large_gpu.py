@@ -75,3 +75,16 @@ def test_two_runs_of_a_large_batch_are_bit_equal_and_replays_too(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want[s]))
         torch.randn(500, 500, device=dev).sum()
+
+
+def test_saved_tensors_that_come_back_with_other_strides(dev):
+    """Hooks may bring an equal tensor of any layout."""
+    import svc_autograd as A
+    g = torch.Generator().manual_seed(4)
+    x, r, dy = (torch.randn(2, 48, 60, generator=g).to(dev).requires_grad_(i < 2) for i in range(3))
+    gamma, beta = torch.ones(48, device=dev), torch.zeros(48, device=dev)
+    want = torch.autograd.grad(A.dropout_add_layernorm(x, r, gamma, beta), (x, r), dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.transpose(1, 2).contiguous().transpose(1, 2) if t.shape == x.shape else t.clone()):
+        y = A.dropout_add_layernorm(x, r, gamma, beta)
+    for a, b in zip(want, torch.autograd.grad(y, (x, r), dy)):
+        assert torch.equal(a, b)
