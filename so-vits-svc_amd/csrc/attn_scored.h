@@ -496,7 +496,7 @@ __device__ __forceinline__ void mul_rows(f32x16 (&out)[DP / 32], const E* lds, i
 // What a forward is for.  0: its output alone; P is rounded to the type once.  1: a 16-bit training pass (out32): the backward's row sums of dO out
 // carry P's rounding into every dS, so P goes in as two operands (bf16, 4096 x 4096 causal at 128 channels: dq 2.35e-3 from the exact one instead of
 // 2.5e-3, where rounding dq and dS alone leaves 2.3e-3).  2: fp32, or a 16-bit pass whose dbias, an fp32 result, will be wanted: as many operands as 24
-// bits take, the library's tanh.
+// bits take, the library's tanh; and caps above SHORT_CAP, for the tanh.
 template <typename E, int MODE> constexpr int P_OPS = sizeof(E) == 4 || MODE == 0 ? 1 : MODE == 1 || __is_same(E, f16_t) ? 2 : 3;
 
 // ---- scores in units of log 2 ------------------------------------------------------------------------------------------------------------
@@ -514,7 +514,10 @@ __device__ __forceinline__ ScoreScale score_scale(const svc_attn_scored_t& a) {
   return s;
 }
 // tanh for the cap.  EXACT (fp32, and where a fp32 gradient of the bias hangs on it): the library's.  Else 1 - 2 / (exp 2x + 1), two
-// transcendental instructions: 1e-7 absolute, so 1e-7 of the cap in a score whose P and result are rounded to 2^-8 or 2^-11.
+// transcendental instructions: 1.5e-7 absolute, so 1.5e-7 of the cap in a score, whose P and result are rounded to 2^-8 or 2^-11.  At a cap of 256 that is
+// an eighth of the smaller rounding; above it (SHORT_CAP) 16-bit types take the library's too (4 x 16 heads of 128, 2049 causal, bf16: 137 us for 205, a training
+// pass 952 us for 1132; at a cap of 2^20 the short form would be off by 0.15).
+constexpr float SHORT_CAP = 256.f;
 template <bool EXACT> __device__ __forceinline__ float cap_tanh(float u, const ScoreScale& sc) {
   if (EXACT) return tanhf(u * sc.cap_in);
   return fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u * sc.cap_exp) + 1.f), 1.f);

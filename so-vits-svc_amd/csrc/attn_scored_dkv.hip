@@ -253,7 +253,7 @@ template <typename E, int DP>
 static void go(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
   const int n_tiles = (a.Tk + NCOL - 1) / NCOL;
   const unsigned grid = (unsigned)grid_of((long long)a.B * a.G, 1, n_tiles);
-  const bool exact = sizeof(E) == 4 || a.dbias;
+  const bool exact = sizeof(E) == 4 || a.dbias || a.softcap > SHORT_CAP;
   if (exact && a.seed) hipLaunchKernelGGL((dkv_kernel<E, DP, true, true>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
   else if (exact) hipLaunchKernelGGL((dkv_kernel<E, DP, true, false>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
   else if (a.seed) hipLaunchKernelGGL((dkv_kernel<E, DP, sizeof(E) == 4, true>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);

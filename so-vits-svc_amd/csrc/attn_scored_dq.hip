@@ -247,7 +247,7 @@ template <typename E, int DP>
 static void go(const svc_attn_scored_t& a, const Ws& w, hipStream_t s) {
   const int n_tiles = (a.Tq + NCOL - 1) / NCOL;
   const unsigned grid = (unsigned)grid_of((long long)a.B * a.G, a.H / a.G, n_tiles);
-  if (sizeof(E) == 4 || a.dbias) hipLaunchKernelGGL((dq_kernel<E, DP, true>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
+  if (sizeof(E) == 4 || a.dbias || a.softcap > SHORT_CAP) hipLaunchKernelGGL((dq_kernel<E, DP, true>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
   else hipLaunchKernelGGL((dq_kernel<E, DP, sizeof(E) == 4>), dim3(grid), dim3(256), 0, s, a, w, n_tiles);
 }
 template <typename E>

@@ -216,7 +216,7 @@ static void launch_fwd(const svc_attn_scored_t& a, hipStream_t s) {
   const int n_tiles = (a.Tq + NCOL - 1) / NCOL;
   const unsigned grid = (unsigned)grid_of((long long)a.B * a.G, a.H / a.G, n_tiles);
   constexpr bool F = sizeof(E) == 4;
-  if (F || a.exact) hipLaunchKernelGGL((fwd_kernel<E, DP, 2>), dim3(grid), dim3(256), 0, s, a, n_tiles);
+  if (F || a.exact || a.softcap > SHORT_CAP) hipLaunchKernelGGL((fwd_kernel<E, DP, 2>), dim3(grid), dim3(256), 0, s, a, n_tiles);
   else if (a.out32) hipLaunchKernelGGL((fwd_kernel<E, DP, F ? 2 : 1>), dim3(grid), dim3(256), 0, s, a, n_tiles);
   else hipLaunchKernelGGL((fwd_kernel<E, DP, F ? 2 : 0>), dim3(grid), dim3(256), 0, s, a, n_tiles);
 }

@@ -261,7 +261,7 @@ template <typename E, int DP>
 static void go(const svc_attn_scored_t& a, const Split& p, hipStream_t s) {
   const dim3 grid((unsigned)((long long)a.B * a.G * p.blocks * p.parts));
   constexpr bool F = sizeof(E) == 4;
-  if (F || a.exact) hipLaunchKernelGGL((split_kernel<E, DP, 2>), grid, dim3(256), 0, s, a, p);
+  if (F || a.exact || a.softcap > SHORT_CAP) hipLaunchKernelGGL((split_kernel<E, DP, 2>), grid, dim3(256), 0, s, a, p);
   else if (a.out32) hipLaunchKernelGGL((split_kernel<E, DP, F ? 2 : 1>), grid, dim3(256), 0, s, a, p);
   else hipLaunchKernelGGL((split_kernel<E, DP, F ? 2 : 0>), grid, dim3(256), 0, s, a, p);
 }

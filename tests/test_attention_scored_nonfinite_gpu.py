@@ -171,6 +171,24 @@ def test_the_largest_fp32_values(dev):
     assert not out[:, :, 1:].any()
 
 
+@pytest.mark.parametrize("T", [50, 150])
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("dt", TYPES)
+def test_caps_far_above_the_scores_change_nothing(dev, dt, dk, T):
+    """cap tanh(a / cap) = a - a^3 / 3 cap^2: at a cap of 2^20 and |a| < 8 that is 1e-10, so capped and uncapped calls agree to their roundings: twice u for
+    the result, and twice u for P (for out) or for dS and D (for gradients), of the sums of absolute values."""
+    from oracle import layer_oracle as O
+    dt = TYPES[dt]
+    q, k, v, do = _inputs(dev, dt, 1, 2, 1, dk, T, T)
+    ref = O.attention(q, k, v, 2, dout=do)
+    a, b = _pass(q, k, v, do, 2), _pass(q, k, v, do, 2, softcap=2.0 ** 20)
+    u = max(torch.finfo(dt).eps / 2, 2.0 ** -24 * 8 * dk)
+    for x, y, n, f in zip((a[0], *a[2:5]), (b[0], *b[2:5]), ("out", "dq", "dk", "dv"), (2, 4, 4, 2)):
+        bound = 2 * u * ref[n].abs() + f * u * ref["mag_" + n] + 2.0 ** -24
+        assert ((x.double() - y.double()).abs().cpu() <= bound).all(), n
+        assert ((y.double().cpu() - ref[n]).abs() <= bound).all(), n
+
+
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
 def test_saved_tensors_that_come_back_at_the_same_address_with_other_strides(dev, dt):
     """Hooks that move saved tensors away and back may be given the old memory again: the backward has to look at the strides, not at the address alone."""
