@@ -589,6 +589,7 @@ struct Ws {
   int2* iv;        // [B][Tq]    visible keys
   int4* tiles;     // [B][ceil(Tq/32)]  {min lo, max hi, max lo, min hi} of 32 queries
   float* gmax;     // [B*H][ceil(Tq/64)]  max |dO|
+  float* vmax;     // [B*G][ceil(Tk/128)]  max |v| of the keys that can be seen (fp16)
   float* bins;     // [B*H][ceil(Tq/32)][2 bias_w + 1]  bias gradient of 32 queries
   long long bytes;
 };
@@ -611,22 +612,35 @@ void launch_dq(const svc_attn_scored_t& a, const Ws& w, hipStream_t s);        /
 void launch_dkv(const svc_attn_scored_t& a, const Ws& w, hipStream_t s);       // attn_scored_dkv.hip
 
 // fp16 operands: dS is multiplied by a power of two that brings the largest |dO| of the key head to [1, 2): gradients of any magnitude then
-// sit in the middle of the type's range (a loss scale of 2^-12 would otherwise leave dS among its subnormals), and |dS| <= 2 P |dO| |v|
-// dk stays below 65504 for |v| up to 250.  The factor is divided out of the fp32 accumulators.
+// sit in the middle of the type's range (a loss scale of 2^-12 would otherwise leave dS among its subnormals).  |dS| = P |Z dP - D| is at most `most` = 2 keep dk
+// max |dO| max |v|: where that would pass 65504 (max |v| above 128 at 128 channels), the power is the largest that keeps it below.  The factor is divided out of the
+// fp32 accumulators.  red: 8 floats.
 template <typename E> __device__ __forceinline__ float operand_scale(const svc_attn_scored_t& a, const Ws& w, int b, int kvh, float* red) {
   if constexpr (!__is_same(E, f16_t)) return 1.f;
-  const int n_tiles = (a.Tq + 63) / 64, rep = a.H / a.G, n = rep * n_tiles;
+  const int n_tiles = (a.Tq + 63) / 64, rep = a.H / a.G, n = rep * n_tiles, nk = (a.Tk + 127) / 128;
   const float* g = w.gmax + ((long long)b * a.H + (long long)kvh * rep) * n_tiles;
-  float m = 0.f;
+  const float* gv = w.vmax + ((long long)b * a.G + kvh) * nk;
+  float m = 0.f, v = 0.f;
   for (int i = threadIdx.x; i < n; i += 256) m = fmaxf(m, g[i]);
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  for (int i = threadIdx.x; i < nk; i += 256) v = fmaxf(v, gv[i]);
+  for (int o = 32; o > 0; o >>= 1) {
+    m = fmaxf(m, __shfl_xor(m, o));
+    v = fmaxf(v, __shfl_xor(v, o));
+  }
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = m;
+    red[4 + (threadIdx.x >> 6)] = v;
+  }
   __syncthreads();
   m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  v = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
   if (!(m > 0.f) || !(m < INFINITY)) return 1.f;
   int e;
   frexpf(m, &e);
-  return ldexpf(1.f, 1 - e);
+  const float f = ldexpf(1.f, 1 - e), keep = a.seed ? 65536.f / (65536.f - rintf(a.p_drop * 65536.f)) : 1.f, most = 2.f * keep * a.dk * m * v;
+  if (!(most * f > 65504.f) || !(most < INFINITY)) return f;
+  frexpf(65504.f / most, &e);
+  return ldexpf(1.f, e - 1);
 }
 
 }  // namespace attn

@@ -20,15 +20,34 @@ static Ws layout(const svc_attn_scored_t& a) {
   w.iv = (int2*)take((long long)a.B * a.Tq * 8);
   w.tiles = (int4*)take(a.B * t32 * 16);
   w.gmax = (float*)take(bh * ((a.Tq + 63) / 64) * 4);
+  w.vmax = (float*)take(a.dtype == SVC_F16 ? (long long)a.B * a.G * ((a.Tk + 127) / 128) * 4 : 0);
   w.bins = (float*)take(a.dbias ? bh * t32 * (2LL * a.bias_w + 1) * 4 : 0);
   w.bytes = o;
   return w;
 }
 
-// ---- rows: D = sum_d dO[d,t] out[d,t], the largest |dO|, and the visible intervals.  64 queries of one head a workgroup ----------
+// ---- rows: D = sum_d dO[d,t] out[d,t], the largest |dO|, and the visible intervals.  64 queries of one head a workgroup; fp16: and the largest |v|, 128
+// keys of one key head a workgroup behind those ----------
 template <typename E>
 __global__ __launch_bounds__(256) void rows_kernel(svc_attn_scored_t a, Ws w, int n_tiles) {
   __shared__ float sum[4][64], big[4][64];
+  if constexpr (__is_same(E, f16_t)) {
+    if ((int)blockIdx.x >= a.B * a.H * n_tiles) {
+      const int nk = (a.Tk + 127) / 128, at = blockIdx.x - a.B * a.H * n_tiles, s = at % nk * 128 + (threadIdx.x & 127), b = at / nk / a.G, kvh = at / nk % a.G;
+      int tbeg, tend, kbeg, kend;
+      live_range(a, b, tbeg, tend, kbeg, kend);
+      float g = 0.f;
+      if (s >= kbeg && s < kend) {
+        const E* v = (const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs + s;
+        for (int d = threadIdx.x >> 7; d < a.dk; d += 2) g = fmaxf(g, fabsf(to_f(v[d * a.v_cs])));
+      }
+      for (int o = 32; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor(g, o));
+      if ((threadIdx.x & 63) == 0) big[threadIdx.x >> 6][0] = g;
+      __syncthreads();
+      if (threadIdx.x == 0) w.vmax[at] = fmaxf(fmaxf(big[0][0], big[1][0]), fmaxf(big[2][0], big[3][0]));
+      return;
+    }
+  }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int bh = blockIdx.x / n_tiles, tile = blockIdx.x % n_tiles, t = tile * 64 + lane;
   const int b = bh / a.H, head = bh % a.H;
@@ -108,7 +127,8 @@ int svc_attn_scored_bwd(const svc_attn_scored_t* a, void* stream) {
   svc::ProfScope prof(s, "attn_scored_bwd", 14.0 * a->B * a->H * (double)a->Tq * a->Tk * a->dk, 0);
   const attn::Ws w = attn::layout(*a);
   const int n64 = (a->Tq + 63) / 64;
-  const dim3 grid((unsigned)(a->B * a->H * n64));
+  const int rows = a->B * a->H * n64, keys = a->dtype == SVC_F16 ? a->B * a->G * ((a->Tk + 127) / 128) : 0;      // (together up to 15 2^20 workgroups)
+  const dim3 grid((unsigned)(rows + keys));
   if (a->dtype == SVC_F32) hipLaunchKernelGGL((attn::rows_kernel<float>), grid, dim3(256), 0, s, *a, w, n64);
   else if (a->dtype == SVC_BF16) hipLaunchKernelGGL((attn::rows_kernel<attn::bf16_t>), grid, dim3(256), 0, s, *a, w, n64);
   else hipLaunchKernelGGL((attn::rows_kernel<attn::f16_t>), grid, dim3(256), 0, s, *a, w, n64);

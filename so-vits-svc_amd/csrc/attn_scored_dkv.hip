@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
   __shared__ float win[2][NCOL + N];
   __shared__ __align__(16) float lses[2][N], rows[2][N];
   __shared__ __align__(16) int2 ivs[2][N];
-  __shared__ float red[4];
+  __shared__ float red[8];
   E* const tiles = (E*)tiles_;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, n = lane & 31, rep = a.H / a.G;
   const Place at = place_of(blockIdx.x, a.B * a.G, 1, n_tiles);

@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 128) ? 2 : 
   __shared__ __align__(16) char tiles_[2 * Staged<E, DP, RB>::BUFS * Staged<E, DP, RB>::SIZE * sizeof(E)];
   __shared__ float win[2][NCOL + N];
   __shared__ float bin_[4][2][NB];
-  __shared__ float red[4];
+  __shared__ float red[8];
   E* const tiles = (E*)tiles_;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, n = lane & 31;
   const Place at = place_of(blockIdx.x, a.B * a.G, a.H / a.G, n_tiles);

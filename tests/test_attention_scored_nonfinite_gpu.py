@@ -189,6 +189,33 @@ def test_caps_far_above_the_scores_change_nothing(dev, dt, dk, T):
         assert ((y.double().cpu() - ref[n]).abs() <= bound).all(), n
 
 
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("size", [100.0, 12000.0])
+def test_large_fp16_values_keep_the_gradients(dev, size, dk, p):
+    """fp16 v of thousands: dS is far inside fp32, and its fp16 operand has to stay inside fp16.  Bounds as in tests/test_attention_scored_gpu.py, with the
+    operand's steps among fp16's subnormals: it is scaled so that the largest |dO| lies in [1, 2), or, where that is less, so that 2 keep dk max |dO| max |v|
+    lies between 32752 and 65504."""
+    import svc_hip as S
+    from oracle import layer_oracle as O
+    q, k, v, do = _inputs(dev, torch.float16, 2, 4, 2, dk, 150, 150)
+    v, do = (v.float() * size).clamp(-60000, 60000).half(), (do.sign() * 1.9 * 2.0 ** -10).half()
+    kw = dict(draw=S.HashDraw(torch.tensor([3], device=dev), 1), p_drop=p) if p else {}
+    ref = O.attention(q, k, v, 4, dout=do, **kw)
+    got = _pass(q, k, v, do, 4, **kw)
+    u = 2.0 ** -11
+    f = 2.0 ** -24 * (4 * (dk + 8) * (1 + ref["score"]) + 150 + 64)
+    top = lambda x: x.double().abs().max().item()  # noqa: E731
+    allowed = 2 / (1 - p) * dk * top(do) * top(v)
+    step = max(top(do), allowed / 32752) * 2.0 ** -25
+    floor = {"out": 300 * 2.0 ** -33 * top(v), "dv": 300 * 2.0 ** -33 * top(do), "dq": 150 * step * top(k) * dk ** -0.5, "dk": 300 * step * top(q) * dk ** -0.5}
+    for x, n, m in zip((got[0], *got[2:5]), ("out", "dq", "dk", "dv"), (1.0, 2.0, 2.0, 1.0)):
+        assert torch.isfinite(x).all(), n
+        bound = u * ref[n].abs() + m * (u + f) * ref["mag_" + n] + floor[n] + 2.0 ** -25
+        worst = ((x.double().cpu() - ref[n]).abs() / bound).max().item()
+        assert worst <= 1, (n, worst)
+
+
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
 def test_saved_tensors_that_come_back_at_the_same_address_with_other_strides(dev, dt):
     """Hooks that move saved tensors away and back may be given the old memory again: the backward has to look at the strides, not at the address alone."""
