@@ -764,7 +764,9 @@ int svc_cmag_bwd_f32(const float* re, const float* im, const float* mag, const f
  * without keys) and out32 [B,H*dk,Tq], contiguous: the output in fp32, from which 16-bit types' backward takes its row sums of dO out.
  * svc_attn_scored_bwd reads q, k, v, out32 (fp32: out), lse, dout and writes dq, dk, dv (contiguous [B, heads*dk, T]) and dbias.  The row sums enter
  * dbias, an fp32 result of any type's call, unrounded: a forward whose dbias will be wanted is asked for with `exact`.  No atomics on memory:
- * results do not vary from run to run.  scale > 0.  ws: svc_attn_scored_ws_bytes(a, backward) bytes, 16-byte aligned, contents undefined before and after.
+ * results do not vary from run to run.  scale > 0.  ws: svc_attn_scored_ws_bytes(a, backward) bytes (0 for sizes that the calls refuse), 16-byte aligned, contents
+ * undefined before and after; with dbias it holds B H ceil(Tq / 32) (2 bias_w + 1) floats among others: 4 items of 16 heads, 8192 queries and distances up to
+ * 8191 are 1.07 GB (a table whose distances end where they matter: 34 MB for bias_w = 256).
  * Built for 1 <= dk <= 128, 0 <= Tq <= Tk < 2^30, B H ceil(Tk / 128) < 5 2^20; with a bias H < 2^16 and bias_w < 2^24.  out shares no memory with the inputs.
  * ---------------------------------------------------------------------------------------------- */
 enum { SVC_F32 = 0, SVC_BF16 = 1, SVC_F16 = 2 };
@@ -804,7 +806,7 @@ int svc_attn_scored_bwd(const svc_attn_scored_t* a, void* stream);
  * gradient are 0 whatever x and r hold there.  r may be NULL.  seed != NULL: dropout of x with svc_dropout_rng_f32's draws of (seed, site) and
  * rate p, recomputed in the backward.  Statistics, sums and gradients in fp32 (the parameters' in fixed order, no atomics).
  * Backward: dx may be NULL (no dropout: it equals dr).  Built for B < 2^16, B ceil(T / 16) < 2^23, C < 2^25; y, dx, dr share no memory with the
- * inputs.  ws: svc_dropout_add_layernorm_ws_bytes(B, C, T) bytes, 16-byte aligned. */
+ * inputs.  ws: svc_dropout_add_layernorm_ws_bytes(B, C, T) bytes (0 for sizes that the calls refuse), 16-byte aligned. */
 typedef struct svc_dropout_add_layernorm_t {
   const void* x;
   const void* r;

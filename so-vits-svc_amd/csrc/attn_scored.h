@@ -581,7 +581,8 @@ __device__ __forceinline__ int wave_max(int v) {
 }
 __device__ __forceinline__ int wave_min(int v) { return -wave_max(-v); }      // (values are positions: never the lowest int)
 
-int check_args(const svc_attn_scored_t* a, bool backward);      // attn_scored_fwd.hip
+int check_sizes(const svc_attn_scored_t* a);                    // attn_scored_fwd.hip
+int check_args(const svc_attn_scored_t* a, bool backward);
 
 // ---- the backward's workspace -----------------------------------------------------------------------------------------------------------
 struct Ws {

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(1024) void dbias_kernel(svc_attn_scored_t a, Ws ws)
 extern "C" {
 
 long long svc_attn_scored_ws_bytes(const svc_attn_scored_t* a, int backward) {
-  if (!a || a->B < 1 || a->Tq < 1 || a->G < 1) return 0;
+  if (!a || attn::check_sizes(a) != SVC_OK || a->B < 1 || a->Tq < 1) return 0;
   return backward ? attn::layout(*a).bytes : attn::split_ws_bytes(*a, attn::split_of(*a));
 }
 

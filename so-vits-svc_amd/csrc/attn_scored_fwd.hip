@@ -180,18 +180,26 @@ __global__ __launch_bounds__(256, X3<E> && DP > 96 ? 1 : 2) void fwd_kernel(svc_
     }
 }
 
-int check_args(const svc_attn_scored_t* a, bool backward) {
+// What the sizes alone decide: the workspace's queries ask this too, before anything is divided or multiplied.
+int check_sizes(const svc_attn_scored_t* a) {
   SVC_REQUIRE(a, "attn_scored: no arguments");
   SVC_REQUIRE(a->dtype >= 0 && a->dtype <= 2, "attn_scored: dtype %d", a->dtype);
   SVC_REQUIRE(a->B >= 0 && a->Tq >= 0 && a->Tq <= a->Tk && a->Tk < (1 << 30), "attn_scored: B=%d Tq=%d Tk=%d (0 <= Tq <= Tk < 2^30)",
               a->B, a->Tq, a->Tk);
   SVC_REQUIRE(a->G >= 1 && a->H >= a->G && a->H % a->G == 0, "attn_scored: %d query heads, %d key heads", a->H, a->G);
   SVC_REQUIRE(a->dk >= 1 && a->dk <= 128, "attn_scored: head size %d (1..128)", a->dk);
+  SVC_REQUIRE(!a->bias || (a->bias_w >= 0 && a->bias_w < (1 << 24) && a->H < 65536 && (a->bias_heads == 1 || a->bias_heads == a->H)),
+              "attn_scored: bias of %d heads, width %d", a->bias_heads, a->bias_w);
+  // (a launch has fewer than 2^32 threads: the widest has three workgroups of 256 for 128 keys of a head; the product of any three ints fits a double's range)
+  const double groups = (double)a->B * a->H * svc::cdiv(a->Tk, 128);
+  SVC_REQUIRE(a->Tq == 0 || groups < 5. * (1 << 20), "attn_scored: %.0f tiles of 128 keys (up to 5 2^20)", groups);
+  return SVC_OK;
+}
+int check_args(const svc_attn_scored_t* a, bool backward) {
+  if (const int rc = check_sizes(a)) return rc;
   SVC_REQUIRE(a->offsets || (a->offset >= 0 && a->offset <= a->Tk - a->Tq), "attn_scored: offset %d with Tq=%d Tk=%d", a->offset, a->Tq, a->Tk);
   SVC_REQUIRE(a->window >= -1 && a->n_docs >= 0 && (a->n_docs == 0 || a->docs), "attn_scored: window %d, %d documents", a->window, a->n_docs);
   SVC_REQUIRE(!a->prefix || (a->causal && a->window < 0), "attn_scored: a prefix goes with a causal mask and no window");
-  SVC_REQUIRE(!a->bias || (a->bias_w >= 0 && a->bias_w < (1 << 24) && a->H < 65536 && (a->bias_heads == 1 || a->bias_heads == a->H)),
-              "attn_scored: bias of %d heads, width %d", a->bias_heads, a->bias_w);
   SVC_REQUIRE(a->scale > 0.f && a->scale < INFINITY && a->softcap >= 0.f && a->softcap < INFINITY, "attn_scored: scale %g, softcap %g", a->scale, a->softcap);
   SVC_REQUIRE(!a->seed || (a->p_drop >= 0.f && a->p_drop <= 0.99f), "attn_scored: dropout rate %g (0..0.99)", a->p_drop);
   if (a->B == 0 || a->Tq == 0) return SVC_OK;
@@ -205,9 +213,6 @@ int check_args(const svc_attn_scored_t* a, bool backward) {
   const long long need = svc_attn_scored_ws_bytes(a, backward);
   SVC_REQUIRE(need == 0 || (a->ws && a->ws_bytes >= need && ((size_t)a->ws & 15) == 0), "attn_scored: workspace of %lld bytes needed, %lld given",
               need, a->ws ? a->ws_bytes : 0LL);
-  // (a launch has fewer than 2^32 threads: the widest has three workgroups of 256 for 128 keys of a head)
-  const long long groups = (long long)a->B * a->H * svc::cdiv(a->Tk, 128);
-  SVC_REQUIRE(groups < (5LL << 20), "attn_scored: %lld tiles of 128 keys (up to 5 2^20)", groups);
   return SVC_OK;
 }
 

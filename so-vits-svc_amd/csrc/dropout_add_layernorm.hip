@@ -499,6 +499,9 @@ static void run(const svc_dropout_add_layernorm_t& a, const Plan& p, bool backwa
   }
 }
 
+// (a launch has fewer than 2^32 threads: 512 for 16 columns, 1024 for 16 channels' sums)
+bool sizes_fit(int B, int C, int T) { return B < 65536 && C < (1 << 25) && (long long)B * ((T + 15LL) / 16) < (1LL << 23); }
+
 int check(const svc_dropout_add_layernorm_t* a, bool backward) {
   SVC_REQUIRE(a, "dropout_add_layernorm: no arguments");
   SVC_REQUIRE(a->dtype >= 0 && a->dtype <= 2, "dropout_add_layernorm: dtype %d", a->dtype);
@@ -506,8 +509,7 @@ int check(const svc_dropout_add_layernorm_t* a, bool backward) {
   SVC_REQUIRE(!a->seed || (a->p >= 0.f && a->p < 1.f), "dropout_add_layernorm: rate %g (0 <= p < 1)", a->p);
   SVC_REQUIRE(a->eps > 0.f, "dropout_add_layernorm: eps %g", a->eps);
   if (a->B == 0 || a->T == 0) return SVC_OK;
-  // (a launch has fewer than 2^32 threads: 512 for 16 columns, 1024 for 16 channels' sums)
-  SVC_REQUIRE((long long)a->B * svc::cdiv(a->T, 16) < (1LL << 23) && a->C < (1 << 25), "dropout_add_layernorm: B=%d C=%d T=%d (built for 2^27 columns, 2^25 channels)",
+  SVC_REQUIRE(sizes_fit(a->B, a->C, a->T), "dropout_add_layernorm: B=%d C=%d T=%d (built for 2^27 columns, 2^25 channels)",
               a->B, a->C, a->T);
   SVC_REQUIRE(a->x && a->gamma && a->beta, "dropout_add_layernorm: x, gamma, beta");
   if (!backward) {
@@ -526,7 +528,7 @@ int check(const svc_dropout_add_layernorm_t* a, bool backward) {
 extern "C" {
 
 long long svc_dropout_add_layernorm_ws_bytes(int B, int C, int T) {
-  return B < 1 || C < 1 || T < 1 ? 0 : 2LL * C * plan_of(B, C, T, true).blocks * 4;
+  return B < 1 || C < 1 || T < 1 || !sizes_fit(B, C, T) ? 0 : 2LL * C * plan_of(B, C, T, true).blocks * 4;
 }
 
 int svc_dropout_add_layernorm_fwd(const svc_dropout_add_layernorm_t* a, void* stream) {
