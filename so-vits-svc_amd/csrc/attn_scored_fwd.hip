@@ -201,6 +201,9 @@ int check_args(const svc_attn_scored_t* a, bool backward) {
   SVC_REQUIRE(a->window >= -1 && a->n_docs >= 0 && (a->n_docs == 0 || a->docs), "attn_scored: window %d, %d documents", a->window, a->n_docs);
   SVC_REQUIRE(!a->prefix || (a->causal && a->window < 0), "attn_scored: a prefix goes with a causal mask and no window");
   SVC_REQUIRE(a->scale > 0.f && a->scale < INFINITY && a->softcap >= 0.f && a->softcap < INFINITY, "attn_scored: scale %g, softcap %g", a->scale, a->softcap);
+  // (the kernels' factors: score_scale)
+  SVC_REQUIRE(a->scale * LOG2E < INFINITY && a->softcap * LOG2E < INFINITY && (a->softcap == 0.f || a->scale / a->softcap * (2.f * LOG2E) < INFINITY),
+              "attn_scored: scale %g with softcap %g: beyond fp32", a->scale, a->softcap);
   SVC_REQUIRE(!a->seed || (a->p_drop >= 0.f && a->p_drop <= 0.99f), "attn_scored: dropout rate %g (0..0.99)", a->p_drop);
   if (a->B == 0 || a->Tq == 0) return SVC_OK;
   SVC_REQUIRE(a->q && a->k && a->v, "attn_scored: q, k, v");

@@ -49,3 +49,12 @@ def test_junction_workspace_of_the_largest_arguments():
     import svc_hip as S
     assert S.lib().svc_dropout_add_layernorm_ws_bytes(8, 200, 5000) == 2 * 200 * 512 * 4
     assert S.lib().svc_dropout_add_layernorm_ws_bytes(65535, (1 << 25) - 1, 1) == 2 * ((1 << 25) - 1) * 65535 * 4
+
+
+@pytest.mark.parametrize("bad", [dict(scale=3e38), dict(softcap=3e38), dict(softcap=1e-40), dict(scale=1e30, softcap=1e-10)], ids=str)
+def test_factors_beyond_fp32_are_refused(bad):
+    """Scores are worked out in units of log 2 from scale log2(e), cap log2(e) and 2 log2(e) scale / cap: an infinite one makes NaN of a score of 0."""
+    import svc_hip as S
+    for fn in (S.lib().svc_attn_scored_fwd, S.lib().svc_attn_scored_bwd):
+        assert fn(ctypes.byref(_attn(**bad)), None) == -1
+        assert b"scale" in S.lib().svc_last_error()
