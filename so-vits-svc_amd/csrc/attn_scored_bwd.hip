@@ -39,6 +39,7 @@ __global__ __launch_bounds__(256) void rows_kernel(svc_attn_scored_t a, Ws w, in
       float g = 0.f;
       if (s >= kbeg && s < kend) {
         const E* v = (const E*)a.v + b * a.v_bs + (long long)kvh * a.dk * a.v_cs + s;
+#pragma unroll 8
         for (int d = threadIdx.x >> 7; d < a.dk; d += 2) g = fmaxf(g, fabsf(to_f(v[d * a.v_cs])));
       }
       for (int o = 32; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor(g, o));

@@ -165,13 +165,6 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
           const int2 w = ivs[cur][32 * rt + pos_of(i, h)];
           x[i] = s >= w.x && s < w.y ? x[i] : 0.f;
         }
-        if (sc.cap) {                                        // (what lies at keys that no query sees may be nan, and so its cap factor, by which 0 is multiplied below)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int2 w = ivs[cur][32 * rt + pos_of(i, h)];
-            th[i] = s >= w.x && s < w.y ? th[i] : 0.f;
-          }
-        }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] = x[i];
@@ -207,24 +200,24 @@ __global__ __launch_bounds__(256, (sizeof(E) == 4 ? DP <= 32 : DP <= 64) ? 2 : 1
         // P (Z dP - D) = (Z P) dP - P D needs no dropped bits, at sixteen registers that the 16-bit kernels lack
         // (64 channels with dropout: 13 spills and 138-149 us against 133; fp32 at 96: 199 us against 217)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float g = fmaf(p[i], dp[i], -(x[i] * rows[cur][32 * rt + pos_of(i, h)]));
-          x[i] = whole || x[i] != 0.f ? g : 0.f;             // (a nan P is not a masked one)
-        }
+        for (int i = 0; i < 16; ++i) dp[i] = fmaf(p[i], dp[i], -(x[i] * rows[cur][32 * rt + pos_of(i, h)]));
       } else {
         if (DROP && (EARLY || a.seed)) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) dp[i] = gone >> i & 1 ? 0.f : dp[i] * keep;
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float g = x[i] * (dp[i] - rows[cur][32 * rt + pos_of(i, h)]);
-          x[i] = whole || x[i] != 0.f ? g : 0.f;             // (a masked entry: 0 whatever dO.v is; a nan P is not one)
-        }
+        for (int i = 0; i < 16; ++i) dp[i] -= rows[cur][32 * rt + pos_of(i, h)];
       }
       if (sc.cap) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
+        for (int i = 0; i < 16; ++i) dp[i] *= fmaf(-th[i], th[i], 1.f);
+      }
+      // a masked entry: 0 whatever dO.v and the cap's factor are (no query need see the key, which may then hold anything); a nan P is not one
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float g = X3<E> ? dp[i] : x[i] * dp[i];
+        x[i] = whole || x[i] != 0.f ? g : 0.f;
       }
       if constexpr (__is_same(E, f16_t)) {
 #pragma unroll
