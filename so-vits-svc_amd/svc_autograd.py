@@ -1012,9 +1012,9 @@ def attention_qkv(qkv, n_heads, emb_rel_k=None, emb_rel_v=None, window=0, mask=N
     return _AttentionQKV.apply(qkv, emb_rel_k, emb_rel_v, mask, n_heads, window or 0, mask_mode, drop_u, float(p_drop))
 
 
-def _places(*tensors):
-    """Where tensors lie, to tell whether saved-tensor hooks brought others back: they may be given an old address with other strides."""
-    return [None if t is None else (t.data_ptr(), t.stride()) for t in tensors]
+def _back(at, t):
+    """Whether saved-tensor hooks brought back the contiguous tensor that lay at `at` (another may be given its address with other strides)."""
+    return t is None or (t.data_ptr() == at and t.is_contiguous())
 
 
 class _AttentionScored(Function):
@@ -1024,18 +1024,19 @@ class _AttentionScored(Function):
     def forward(ctx, q, k, v, bias, n_heads, opts, sides, draw):
         args, dev = S._attn_scored_args(q, k, v, n_heads, bias, draw=draw, **opts, **sides)
         out, lse, out32 = S._scored_forward(args, dev, q, ctx.needs_input_grad[3])
-        kept = (q, k, v, bias, lse, out if out32 is None else out32, *sides.values())
-        ctx.save_for_backward(*kept)
-        ctx.cfg = (args, dev, n_heads, opts, list(sides), draw, _places(*kept))
+        ctx.save_for_backward(q, k, v, bias, lse, out if out32 is None else out32, *sides.values())
+        ctx.cfg = (args, dev, n_heads, opts, list(sides), draw, [t.data_ptr() for t in sides.values()])
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        kept = ctx.saved_tensors
-        q, k, v, bias, lse, out, *sides = kept
+        q, k, v, bias, lse, out, *sides = ctx.saved_tensors
         args, dev, n_heads, opts, names, draw, places = ctx.cfg
-        if _places(*kept) != places:      # saved-tensor hooks brought other tensors back
+        if not ((args.q, args.q_bs, args.q_cs) == (q.data_ptr(), *S._bct_strides(q)) and (args.k, args.k_bs, args.k_cs) == (k.data_ptr(), *S._bct_strides(k)) and
+                (args.v, args.v_bs, args.v_cs) == (v.data_ptr(), *S._bct_strides(v)) and _back(args.bias, bias) and _back(args.lse, lse) and
+                _back(args.out32 if args.dtype else args.out, out) and all(map(_back, places, sides))):
+            # saved-tensor hooks brought other tensors back
             return (*S.attention_scored_bwd(dout, q, k, v, out, lse, n_heads, bias=bias, draw=draw, want_dbias=ctx.needs_input_grad[3], **opts,
                                             **dict(zip(names, sides))), None, None, None, None)
         return (*S._scored_backward(args, dev, dout, q, k, v, bias if ctx.needs_input_grad[3] else None), None, None, None, None)
@@ -1061,16 +1062,17 @@ class _DropoutAddLayerNorm(Function):
         x, r = _c(x), None if r is None else _c(r)
         y, st = S._junction_forward(args, dev, x, r, True)
         ctx.save_for_backward(x, r, gamma, beta, st, mask)
-        ctx.cfg = (args, dev, draw, p, eps, _places(gamma, beta, st, mask))
+        ctx.cfg = (args, dev, draw, p, eps)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, r, gamma, beta, st, mask = ctx.saved_tensors
-        args, dev, draw, p, eps, places = ctx.cfg
-        if _places(gamma, beta, st, mask) != places:      # saved-tensor hooks brought other tensors back
+        args, dev, draw, p, eps = ctx.cfg
+        if not (_back(args.gamma, gamma) and _back(args.mean, st) and _back(args.mask, mask)):      # saved-tensor hooks brought other tensors back
             args, dev = S._junction_args(x, r, gamma, beta, mask, draw, p, eps)
+            st = st.contiguous()
             args.mean, args.rstd = st[0].data_ptr(), st[1].data_ptr()
         return (*S._junction_backward(args, dev, dy, _c(x), None if r is None else _c(r)), None, None, None, None)
 

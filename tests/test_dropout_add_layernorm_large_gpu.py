@@ -88,3 +88,23 @@ def test_saved_tensors_that_come_back_with_other_strides(dev):
         y = A.dropout_add_layernorm(x, r, gamma, beta)
     for a, b in zip(want, torch.autograd.grad(y, (x, r), dy)):
         assert torch.equal(a, b)
+
+
+def test_saved_statistics_that_come_back_at_the_same_address_with_other_strides(dev):
+    import svc_autograd as A
+    g = torch.Generator().manual_seed(4)
+    x, r, dy = (torch.randn(2, 48, 60, generator=g).to(dev).requires_grad_(i < 2) for i in range(3))
+    gamma, beta = torch.ones(48, device=dev), torch.zeros(48, device=dev)
+    want = torch.autograd.grad(A.dropout_add_layernorm(x, r, gamma, beta), (x, r), dy)
+
+    def unpack(t):
+        if t.shape != (2, 2, 60):           # mean and rstd
+            return t
+        turned = t.transpose(0, 1).contiguous()
+        t.view(-1).copy_(turned.view(-1))
+        return t.view(-1).view(2, 2, 60).transpose(0, 1)
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = A.dropout_add_layernorm(x, r, gamma, beta)
+    for a, b in zip(want, torch.autograd.grad(y, (x, r), dy)):
+        assert torch.equal(a, b)
