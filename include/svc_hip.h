@@ -745,7 +745,7 @@ int svc_cmag_bwd_f32(const float* re, const float* im, const float* mag, const f
  *   p outside [0, len)  none
  *   n_docs > 0          those of its document, [docs[b][n], docs[b][n+1]) with n_docs + 1 non-decreasing boundaries per item; none when
  *                       p lies in no document
- *   causal              s <= p, and with `prefix` also s < start + prefix (start = the document's or 0; prefix[b], or prefix[b][n]
+ *   causal              s <= p, and with `prefix` also s < start + prefix (start = the document's first boundary, of either sign, or 0; prefix[b], or prefix[b][n]
  *                       with documents): a bidirectional front
  *   window >= 0         |s - p| <= window (not together with prefix); -1: none
  * What lies at keys that no query of a tile sees (unwritten cache behind `lengths`, other documents' tails) is never used.

@@ -127,8 +127,8 @@ __device__ __forceinline__ int2 visible(const svc_attn_scored_t& a, int b, int l
     }
     if (l < 1 || l > a.n_docs) return make_int2(0, 0);
     n = l - 1;
-    start = max(d[n], 0);
-    lo = start;
+    start = d[n];                       // (before the key axis, in a cache whose oldest positions were dropped: a prefix counts from there)
+    lo = max(start, 0);
     hi = min(hi, d[n + 1]);
   }
   if (a.causal) {
