@@ -1,7 +1,7 @@
 // attn_scored_bwd.hip — svc_attn_scored_bwd: gradients of svc_attn_scored_fwd.  Two passes, each recomputing the scores it needs (a walk over
 // keys for dq and the bias, a walk over queries for dk and dv): seven products instead of five, and in exchange no atomics on
 // memory, so that results do not vary from run to run, and no copies of dq that a further launch would have to add up.  What stands around the passes is
-// read once and small: the row sums 48 us at 4 x 16 x 128 x 4096 bf16 (dO and out32, 201 MB: 4.2 TB/s), 13-19 us elsewhere; the bias 5 us.
+// read once and small: the row sums 49 us at 4 x 16 x 128 x 4096 bf16 (dO and out32, 201 MB: 4.1 TB/s), 11 to 19 us elsewhere; the bias 5 us.
 #include "attn_scored.h"
 
 namespace attn {

@@ -3,8 +3,9 @@
 // dv[:, s] = sum_t Z P dO[:, t], dk[:, s] = sum_t dS q[:, t]: four products, k's and v's columns and both results in registers, the query heads that share a
 // key head one after the other, so that their sum needs no second pass.  At 128 channels that is a wave a SIMD (376 registers): the vector unit's part
 // (1900 cycles of the 32 x 32 scores, against 1024 of the matrix unit) then stands beside the matrix unit's only as far as the compiler interleaves
-// them.  Measured: bf16, 128 channels, 16 query and 4 key heads, 4 x 4096 x 4096 causal with a cap 1040 us = 530 TFLOP/s of its four products; bf16,
-// 64 channels, 9 documents in 4099 with bias and dropout 133 us; fp16, window of 128 in 1501 96 us; fp32, 96 channels, 16 ragged items of up to 790 198 us.
+// them.  Short walks wait behind loads and barriers (documents 52 %, windows 57 % of the waves' cycles).  Measured (kernel traces of passes one behind the other): bf16,
+// 128 channels, 16 query and 4 key heads, 4 x 4096 x 4096 causal with a cap 1038 to 1043 us = 528 TFLOP/s of its four products; bf16,
+// 64 channels, 9 documents in 4099 with bias and dropout 130 us; fp16, window of 128 in 1501 92 us; fp32, 96 channels, 16 ragged items of up to 790 190 us.
 #include "attn_scored.h"
 
 namespace attn {

@@ -1,9 +1,10 @@
 // attn_scored_dq.hip — svc_attn_scored_bwd's walk over the keys: dq and the bias gradient.
 //
 // P = exp2(x - lse) again from q and k, dP = Z (dO.v), dS = P (dP - D): three products, with q's and dO's columns in registers throughout.  The vector
-// unit bounds it (scores as in the forward, and the mask, D and cap factors of dS).  Measured: bf16, 128 channels, 4 x 16 heads, 4096 x 4096 causal with a
-// cap 560 us = 735 TFLOP/s of its three products; bf16, 64 channels, 9 documents in 4099 with bias and dropout 71 us; fp16, window of 128 in 1501 with
-// the bias's gradient 95 us; fp32, 96 channels, 16 ragged items of up to 790 131 us.
+// unit bounds it on long rows (scores as in the forward, and the mask, D and cap factors of dS); on short walks loads and barriers do (waits 40 to 43 % of the waves'
+// cycles).  Measured (kernel traces of passes one behind the other): bf16, 128 channels, 4 x 16 heads, 4096 x 4096 causal with a
+// cap 566 to 572 us = 720 to 728 TFLOP/s of its three products; bf16, 64 channels, 9 documents in 4099 with bias and dropout 68 us; fp16, window of 128 in 1501 with
+// the bias's gradient 88 us; fp32, 96 channels, 16 ragged items of up to 790 123 us.
 #include "attn_scored.h"
 
 namespace attn {

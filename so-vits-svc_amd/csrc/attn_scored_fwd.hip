@@ -5,9 +5,10 @@
 // (4 dk operations a visible pair) with the softmax between them in the registers of the first one's accumulator.  At 64 and 128 channels the vector
 // unit is the bound, not the matrix unit: 16 scores a lane cost 32 to 48 transcendental cycles and 8 to 30 ordinary instructions each (cap, bias, mask,
 // draws), the products 512 to 1024 cycles for all; two waves a SIMD overlap the two.  128 queries a workgroup share every k and v tile through LDS; a
-// tile's loads are in flight while the one before is worked on.  Measured (kernel alone): bf16, 128 channels, 4 x 16 heads, 4096 x 4096 causal with a
-// cap 505 us = 545 TFLOP/s; a call of 2049 x 2049 with a prefix 145 us = 500; bf16, 64 channels, 9 documents in 4099 with bias and dropout 60 us; fp16, window
-// of 128 in 1501 58 us; fp32, 96 channels, 16 ragged items of up to 790 with dropout 92 us.
+// tile's loads are in flight while the one before is worked on.  Measured (kernel traces of passes one behind the other): bf16, 128 channels, 4 x 16 heads,
+// 4096 x 4096 causal with a cap 511 to 518 us = 531 to 538 TFLOP/s; 2049 x 2049 with a prefix 156 us, and 145 a call = 502 without the tracer; bf16, 64 channels,
+// 9 documents in 4099 with bias and dropout 59 us; fp16, window of 128 in 1501 56 us; fp32, 96 channels, 16 ragged items of up to 790 with dropout 88 us.  The short
+// walks of documents and windows wait a third of the waves' cycles.
 #include "attn_scored.h"
 
 namespace attn {
@@ -16,7 +17,9 @@ namespace attn {
 template <typename E, int DP, int MODE>
 __global__ __launch_bounds__(256, X3<E> && DP > 96 ? 1 : 2) void fwd_kernel(svc_attn_scored_t a, int n_tiles) {
   constexpr int N = Tile<E>::N, RT = Tile<E>::RT;
-  // a maximum that grows by less than this (a factor 2^LAZY in P) leaves the accumulators as they are: P stays far from any type's range
+  // a maximum that grows by less than this (a factor 2^LAZY in P) leaves the accumulators as they are: P stays far from any type's range.  (Where P is rounded
+  // once, the price is that a row's largest P, 1 against its own maximum, is rounded like the others: prompt of 2049 in bf16 2.3e-3 from 64 bits, of which 1.7e-3 is the
+  // output's own rounding.)
   constexpr float LAZY = __is_same(E, f16_t) ? 4.f : 8.f;
   __shared__ __align__(16) char tiles_[2 * Staged<E, DP>::BUFS * Staged<E, DP>::SIZE * sizeof(E)];
   __shared__ float win[2][NCOL + N];

@@ -4,8 +4,9 @@
 // that shared key heads are read once — and one of `parts` equal parts of the keys they see; its four waves take tiles of it in turn, each through LDS
 // of its own, with no barrier until their results are joined.  Bandwidth is the bound: the next tile's loads (16 KB a wave at 128 channels) are in
 // flight while a tile is worked on.  With more than one part the partial maxima, sums and outputs go through the workspace and a second launch.
-// Measured: 16 streams, 16 query and 4 key heads of 128 channels, caches of 8191 keys of different fill, bf16: 54 us = 3.8 TB/s, and 6.6 us to join the
-// parts; 2 heads of 96 channels, 862 keys, fp32: 19 + 4 us, latency: two launches, and a wave's two tiles one after the other.
+// Measured: 16 streams, 16 query and 4 key heads of 128 channels, caches of 8191 keys of different fill, bf16: 54 us = 3.8 TB/s on one set of caches, 63 on two in
+// turn, and 7 us to join the parts; 2 heads of 96 channels, 862 keys, fp32: 19 + 4 us, latency of 32 waves: the matrix instructions, of whose 32 columns a single query
+// uses one, take 22 % of a wave's cycles, the vector unit 17 %, waits 36 %; and two launches.
 #include "attn_scored.h"
 
 namespace attn {

@@ -4,10 +4,10 @@
 // The backward keeps nothing but mean and rstd: h = r + dropout(x) is recomputed from x, r and the counter draws, which moves the same bytes as
 // storing h would (one write and one read against two reads in place of one) and takes no memory.
 //
-// Measured, 32 x 768 x 1499 bf16 with dropout: forward 91 us (221 MB, 2.4 TB/s), backward 188 us (368 MB, 2.0 TB/s).  The draws are the bound: two 64-bit
-// multiplications an element, 6 quarter-rate instructions of about 40; with the rest of the arithmetic 72 of the forward's us and 86 of the backward's are
-// vector instructions, and a tile's loads, sums and stores stand one behind the other in each workgroup.  16 x 192 x 790 fp32: 13 and 19 us, a tile's
-// own length; 8 x 1001 x 2047 fp16 without dropout: 42 and 69 us (98 and 131 MB).
+// Measured, 32 x 768 x 1499 bf16 with dropout: forward 91 to 95 us (221 MB, 2.3 TB/s), backward 181 to 190 us (368 MB, 2.0 TB/s).  Vector instructions take 65 % of the
+// forward's cycles (the draws: two 64-bit multiplications an element, 6 quarter-rate instructions of about 40) and 37 % of the backward's; the rest are waits, because a
+// tile's loads, sums and stores stand one behind the other in each workgroup.  16 x 192 x 790 fp32: 14 and 19 us, a tile's
+// own length; 8 x 1001 x 2047 fp16 without dropout: 44 and 69 us (98 and 131 MB).
 #include "common.h"
 
 namespace {
