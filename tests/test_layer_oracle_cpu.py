@@ -35,3 +35,26 @@ def test_operands_of_two_parts_would_fail_the_norm(H, G, dk, Tq, Tk, kw):
     for n in ("out", "dq", "dk", "dv"):
         err = ((a[n] - b[n]).norm() / a[n].norm()).item()
         assert err > 32 * 2.0 ** -24, (n, err)
+
+
+def test_p_in_one_bf16_operand_would_fail_the_table_gradients_norm(monkeypatch):
+    """The table's gradient holds D = sum dO out: with P in one bf16 operand it is 1.4e-3 of its norm off, far above 32 x 2^-24; two leave about that bound (1.5e-6),
+    three 2e-9."""
+    g = torch.Generator().manual_seed(11)
+    q, k, v, do = (x * torch.randn(2, n * 96, 200, generator=g).bfloat16().float() for x, n in ((1.5, 2), (1, 1), (1, 1), (1, 2)))
+    bias = 0.7 * torch.randn(2, 81, generator=g)
+    want = O.attention(q, k, v, 2, dout=do, bias=bias)["dbias"]
+    plain, err = torch.einsum, {}
+    for n in (1, 3):
+        def einsum(eq, a, b):
+            if eq == "bhts,bhds->bhdt":                     # out = P v
+                whole, rest = torch.zeros_like(a), a
+                for _ in range(n):
+                    part = rest.float().bfloat16().double()
+                    whole, rest = whole + part, rest - part
+                a = whole
+            return plain(eq, a, b)
+        monkeypatch.setattr(torch, "einsum", einsum)
+        err[n] = ((O.attention(q, k, v, 2, dout=do, bias=bias)["dbias"] - want).norm() / want.norm()).item()
+        monkeypatch.setattr(torch, "einsum", plain)
+    assert err[1] > 100 * 32 * 2.0 ** -24 and err[3] < 2.0 ** -24, err
