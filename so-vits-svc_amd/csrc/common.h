@@ -45,6 +45,9 @@ inline int check_launch(const char* what) {
     }                                   \
   } while (0)
 
+// core.hip: fills `bytes` (a multiple of 4) of device memory with 0 by a kernel.  Never hipMemsetAsync: a memset recorded into a captured graph has left other
+// values than 0 on replays after the first, under gradients that are then added to by atomics.
+void zero(void* p, size_t bytes, hipStream_t s);
 // conv1d_strip.hip: long-sequence dense conv, one workgroup per CU; returns 1 when the shape is not one of its shapes
 int conv1d_strip_try(const svc_conv1d_args& a, hipStream_t s, bool dry = false);
 // ConvTranspose1d weight layout: true = phases as rows [Cin][M][u*CoutP] (row = co*u + phase), one dense convolution;

@@ -692,16 +692,8 @@ extern "C" int svc_conv1d_wgrad_f32(const svc_wgrad_args* ap, void* stream) {
     snprintf(pname, sizeof(pname), "conv1d_wgrad");
   svc::ProfScope prof(s, pname, flop, 4.0 * a.B * ((double)a.Ca * a.TA + (double)a.Cb * a.TB));
   if (!a.accumulate) {
-    if (hipMemsetAsync(a.G, 0, sizeof(float) * (size_t)a.Ca * a.Cb * a.KS, s) != hipSuccess) {
-      svc::set_error("wgrad: memset failed");
-      return SVC_ERR_HIP;
-    }
-  }
-  if (a.dbias && !a.accumulate) {
-    if (hipMemsetAsync(a.dbias, 0, sizeof(float) * (size_t)a.Ca, s) != hipSuccess) {
-      svc::set_error("wgrad: memset failed");
-      return SVC_ERR_HIP;
-    }
+    svc::zero(a.G, sizeof(float) * (size_t)a.Ca * a.Cb * a.KS, s);
+    if (a.dbias) svc::zero(a.dbias, sizeof(float) * (size_t)a.Ca, s);
   }
   if (a.Ca <= 32 && a.Cb <= 32) {
     WgSP q;

@@ -86,6 +86,18 @@ static void drain() {
   g_pending.clear();
 }
 
+// One thread for four words, up to 2048 workgroups (8 a CU) that walk what is more.
+__global__ __launch_bounds__(256) void zero_kernel(unsigned* p, size_t words) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i * 4 < words; i += (size_t)gridDim.x * 256)
+#pragma unroll
+    for (size_t j = i * 4; j < i * 4 + 4; ++j)
+      if (j < words) p[j] = 0u;
+}
+void zero(void* p, size_t bytes, hipStream_t s) {
+  const size_t words = bytes / 4, need = (words + 1023) / 1024;
+  if (words) hipLaunchKernelGGL(zero_kernel, dim3((unsigned)(need < 2048 ? need : 2048)), dim3(256), 0, s, (unsigned*)p, words);
+}
+
 }  // namespace svc
 
 extern "C" {

@@ -221,10 +221,8 @@ extern "C" int svc_snake_alias_bwd_f32(const float* x, const float* dy, const fl
   Taps tp;
   for (int k = 0; k < 12; ++k) tp.f[k] = taps_host[k];
   hipStream_t s = (hipStream_t)stream;
-  if (hipMemsetAsync(dalpha, 0, sizeof(float) * C, s) != hipSuccess || hipMemsetAsync(dbeta, 0, sizeof(float) * C, s) != hipSuccess) {
-    svc::set_error("snake_alias_bwd: memset failed");
-    return SVC_ERR_HIP;
-  }
+  svc::zero(dalpha, sizeof(float) * C, s);
+  svc::zero(dbeta, sizeof(float) * C, s);
   svc::ProfScope ps(s, "snake_alias_bwd", 0.0, 12.0 * B * C * (double)T);
   hipLaunchKernelGGL(snake_alias_bwd_kernel, dim3(svc::cdiv(T, SA_TILE), C, B), dim3(SA_THREADS), 0, s, x, dy, alpha, beta, tp,
                      dx, dalpha, dbeta, x_bs, x_cs, g_bs, g_cs, d_bs, d_cs, T);

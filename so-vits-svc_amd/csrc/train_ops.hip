@@ -872,10 +872,7 @@ int svc_gconv1d_wgrad_f32(const float* dy, const float* x, float* dw, int B, int
   const int NKQ = (KS + GW_KPT - 1) / GW_KPT;
   const size_t lds = sizeof(float) * ((size_t)Og * GW_PD + (size_t)Cg * ((GW_TT - 1) * stride + KS));
   if (g_gconv_version == 2 && (Og == 4 || Og == 16) && Cg == 4 && Og * Cg * NKQ <= 256 && lds <= 60 * 1024) {
-    if (hipMemsetAsync(dw, 0, sizeof(float) * (size_t)Cout * Cg * KS, (hipStream_t)stream) != hipSuccess) {
-      svc::set_error("gconv_wgrad: memset failed");
-      return SVC_ERR_HIP;
-    }
+    svc::zero(dw, sizeof(float) * (size_t)Cout * Cg * KS, (hipStream_t)stream);
     const int total = B * svc::cdiv(Tout, GW_TT);
     const int n_chunks = std::max(1, std::min(total, 1024 / groups));
     const dim3 grid(n_chunks, groups);

@@ -453,11 +453,8 @@ int svc_nsf_linear_fwd_f32(const float* waves, const float* w, const float* b0, 
 int svc_nsf_linear_bwd_f32(const float* waves, const float* har, const float* dhar, float* dw, float* db, long long n, int H,
                            void* stream) {
   SVC_REQUIRE(waves && har && dhar && dw && db && n > 0 && H > 0 && H <= 16, "nsf_linear_bwd: bad args");
-  if (hipMemsetAsync(dw, 0, sizeof(float) * H, (hipStream_t)stream) != hipSuccess ||
-      hipMemsetAsync(db, 0, sizeof(float), (hipStream_t)stream) != hipSuccess) {
-    svc::set_error("nsf_linear_bwd: memset failed");
-    return SVC_ERR_HIP;
-  }
+  svc::zero(dw, sizeof(float) * H, (hipStream_t)stream);
+  svc::zero(db, sizeof(float), (hipStream_t)stream);
   const unsigned grid = (unsigned)std::min<long long>((n + 255) / 256, 512);
   hipLaunchKernelGGL(nsf_linear_bwd_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, waves, har, dhar, dw, db, n, H);
   return svc::check_launch("nsf_linear_bwd");
@@ -740,10 +737,7 @@ int svc_stft_frame_f32(const float* y, const float* win, float* frames, int B, i
 int svc_stft_frame_bwd_f32(const float* dframes, const float* win, float* dy, int B, int L, int NF, int nfft, int hop, int pad,
                            void* stream) {
   SVC_REQUIRE(dframes && win && dy && B > 0 && L > pad && NF > 0, "stft_frame_bwd: bad args");
-  if (hipMemsetAsync(dy, 0, sizeof(float) * (size_t)B * L, (hipStream_t)stream) != hipSuccess) {
-    svc::set_error("stft_frame_bwd: memset failed");
-    return SVC_ERR_HIP;
-  }
+  svc::zero(dy, sizeof(float) * (size_t)B * L, (hipStream_t)stream);
   hipLaunchKernelGGL(stft_frame_bwd_kernel, dim3(svc::cdiv(nfft, 256), NF, B), dim3(256), 0, (hipStream_t)stream, dframes, win,
                      dy, L, NF, nfft, hop, pad);
   return svc::check_launch("stft_frame_bwd");
@@ -810,10 +804,7 @@ int svc_spectral_norm_bwd_f32(const float* W, const float* u, const float* v, co
                               double* dot_ws, int R, int K, void* stream) {
   SVC_REQUIRE(W && u && v && sigma && g && dW && dot_ws && R > 0 && K > 0, "spectral_norm_bwd: bad args");
   hipStream_t s = (hipStream_t)stream;
-  if (hipMemsetAsync(dot_ws, 0, sizeof(double), s) != hipSuccess) {
-    svc::set_error("spectral_norm_bwd: memset failed");
-    return SVC_ERR_HIP;
-  }
+  svc::zero(dot_ws, sizeof(double), s);
   const long long n = (long long)R * K;
   const unsigned grid = (unsigned)std::min<long long>((n + 255) / 256, 1024);
   hipLaunchKernelGGL(sn_dot_kernel, dim3(grid), dim3(256), 0, s, g, W, dot_ws, n);

@@ -58,3 +58,13 @@ def test_factors_beyond_fp32_are_refused(bad):
     for fn in (S.lib().svc_attn_scored_fwd, S.lib().svc_attn_scored_bwd):
         assert fn(ctypes.byref(_attn(**bad)), None) == -1
         assert b"scale" in S.lib().svc_last_error()
+
+
+def test_no_kernel_source_records_a_memset():
+    """What a caller may capture clears memory by a kernel (svc::zero)."""
+    import os
+    import re
+    d = os.path.join(ROOT, "so-vits-svc_amd", "csrc")
+    for f in sorted(os.listdir(d)):
+        if f.endswith((".hip", ".h")):
+            assert not re.search(r"hipMemset\w*\s*\(", open(os.path.join(d, f)).read()), f

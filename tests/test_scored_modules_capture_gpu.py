@@ -107,3 +107,42 @@ def test_block_length_without_a_mask_cuts_nothing(dev):
         assert torch.equal(mod(x, x), everything)
         cut = mod(x, x, attn_mask=torch.ones(1, 1, 50, 50, device=dev))
         assert torch.equal(cut, mod(x, x, mask_mode=MASK_NONE)) and not torch.equal(cut, everything)
+
+
+def test_a_training_pass_in_a_graph_between_eager_passes_of_another_length(dev):
+    """Forward and gradients of a stack captured at one length (its backward reads the pass's own table), replayed on new data between eager training passes
+    and allocations.  Weight gradients are combined with atomics: equal up to their order."""
+    from modules.attentions import FFT
+    torch.manual_seed(9)
+    fft, other = (FFT(64, 128, 2, n_layers=2, kernel_size=3, proximal_bias=True).to(dev).train() for _ in range(2))
+    other.load_state_dict(fft.state_dict())
+    params = [p for n, p in fft.named_parameters() if not n.endswith("conv_k.bias")]      # (whose gradient is rounding alone)
+    twins = [p for n, p in other.named_parameters() if not n.endswith("conv_k.bias")]
+    data = [torch.randn(2, 64, 90, device=dev) for _ in range(3)]
+    m, way = {T: torch.ones(2, 1, T, device=dev) for T in (90, 130)}, {T: torch.randn(2, 64, T, device=dev) for T in (90, 130)}
+
+    def step(net, ps, x):
+        y = net(x, m[x.shape[2]])
+        return [y, *torch.autograd.grad((y * way[x.shape[2]]).sum(), [x, *ps])]
+
+    want = [[t.detach().clone() for t in step(other, twins, x.clone().requires_grad_())] for x in data]
+    held = data[0].clone().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(fft, params, held)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        got = step(fft, params, held)
+    for i in (1, 2, 0, 1):
+        step(other, twins, torch.randn(2, 64, 130, device=dev).requires_grad_())
+        junk = [torch.full((n,), 1e4, device=dev) for n in range(100, 700, 20)]
+        with torch.no_grad():
+            held.copy_(data[i])
+        gr.replay()
+        torch.cuda.synchronize()
+        assert len(junk) == 30
+        for a, b in zip(got, want[i]):
+            assert (a - b).abs().max() <= 1e-4 * b.abs().max().clamp(min=1e-6)
