@@ -1420,8 +1420,8 @@ class PlanSets:
 
 class ZeroSlab:
     """Pre-zeroed storage for the atomically accumulated outputs of one training iteration (weight / bias gradients of
-    svc_conv1d_wgrad_f32): `take` hands out zero-filled views, `reset` re-zeroes what was handed out with ONE memset per
-    chunk.  Replaces one hipMemsetAsync per gradient tensor (585 per iteration of the B=16 GAN step, 2.9 ms of 5 us
+    svc_conv1d_wgrad_f32): `take` hands out zero-filled views, `reset` re-zeroes what was handed out with ONE fill per
+    chunk.  Replaces one clearing launch per gradient tensor (585 per iteration of the B=16 GAN step, 2.9 ms of 5 us
     launches, profiles/r01_k_train_aten_op_census.txt).  Off unless a training loop turns it on (train.TrainStep): a view
     stays valid only until the next reset, i.e. until the optimizer has consumed the gradients of the iteration."""
 
@@ -1462,7 +1462,7 @@ _SLAB_ON = os.environ.get("SVC_WGRAD_SLAB", "1") != "0"
 
 
 def wgrad_zeros(shape, device):
-    """Zero-initialised gradient buffer: a slab view when the slab is active (then no per-tensor memset is needed)."""
+    """Zero-initialised gradient buffer: a slab view when the slab is active (then no clearing per tensor is needed)."""
     if wgrad_slab.active and _SLAB_ON:
         return wgrad_slab.take(shape, device), True
     return torch.empty(tuple(shape), device=device, dtype=torch.float32), False

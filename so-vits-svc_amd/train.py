@@ -242,7 +242,7 @@ class TrainStep:
 
     def _seg_d(self, items, noise=None):
         """Generator forward + the discriminator step up to (and including) its backward (train.py:151-194)."""
-        # weight / bias gradients of this iteration accumulate into one pre-zeroed slab (one memset instead of ~585)
+        # weight / bias gradients of this iteration accumulate into one pre-zeroed slab (one fill instead of ~585)
         S.wgrad_slab.active = True
         S.wgrad_slab.reset()
         c, f0, spec, y, spk, lengths, uv, volume = items
