@@ -99,11 +99,11 @@ class MultiHeadAttention(nn.Module):
         raise NotImplementedError("attention mask is neither all-ones, causal nor an outer product of a padding mask")
 
     def _scored_options(self, mask_mode, mask_vec, T, device, table=None, masked=True):
-        """The options of svc_hip.attention_scored behind this module's: the bias -log1p(|i - j|) as a table over distances (`table`: the one of
-        this pass, where a stack has made it for all its layers), block_length as a
-        window where the call has a mask (:223-229), the padding mask as lengths.  The padding mask must be a sequence mask (not 0, then 0: commons.sequence_mask), which costs a look from
-        the host (`_scored_attention`: while a graph is captured); padded queries
-        give 0 where the reference spreads them over all keys (their rows are masked behind every attention layer)."""
+        """The options of svc_hip.attention_scored behind this module's: the bias -log1p(|i - j|) as a table over distances (`table`: the one of this
+        pass, where a stack has made it for all its layers), block_length as a window where the call has a mask (:223-229), the padding mask as lengths.
+        The padding mask must be a sequence mask (not 0, then 0: commons.sequence_mask); the look at it waits for the device, and where a graph is being
+        captured `_scored_attention` stands in for it.  Padded queries give 0 where the reference spreads them over all keys (their rows are masked
+        behind every attention layer)."""
         opts = {"causal": mask_mode == MASK_CAUSAL, "window": self.block_length if masked else None}
         if mask_mode == MASK_PADDING:
             gone = mask_vec == 0
